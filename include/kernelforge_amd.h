@@ -487,6 +487,107 @@ int kf_fa_bwd(const void* q, const void* k, const void* v, const void* o,
               int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv,
               int64_t D, float scale, int causal, int dtype, kf_stream_t stream);
 
+/* ------------------------------------------------------------------ */
+/* Paged 8-bit key/value cache                                         */
+/* ------------------------------------------------------------------ */
+
+/*
+ * A cache of `blocks` blocks of T = block_tokens tokens (16, 32, 64 or 128)
+ * for Hkv heads of dim D (a multiple of 16, at most 256), in 8 bits with one
+ * fp32 scale for the keys and one for the values of a block and head:
+ *   key_cache   [blocks, Hkv, T, D]
+ *   value_cache [blocks, Hkv, T/16, D, 16]   the 16 tokens of a group innermost
+ *   key_scale, value_scale [blocks, Hkv]
+ * An element is its code times its scale.  Token p of a request lies in slot
+ * p mod T of the block that entry p / T of the request's table row names; slot
+ * s of the cache is slot s mod T of block s / T.  The reference has no cache.
+ */
+typedef enum kf_cache_dtype {
+    KF_CACHE_E4M3 = 0, /* OCP e4m3: largest value 448, no infinities */
+    KF_CACHE_INT8 = 1  /* largest magnitude written 127 */
+} kf_cache_dtype;
+
+/*
+ * Block tables and slots of one step, from the lengths.  Request b holds
+ * o = context_lens[b] tokens and gets n = query_lens[b] new ones (negative
+ * counts read as 0):
+ *   query_starts[0] = 0, query_starts[b+1] = min(query_starts[b] + n, total_tokens),
+ *   context_lens_out[b] = o + query_starts[b+1] - query_starts[b].
+ * The blocks it lacks are taken from free_blocks[*free_used ...] in order of b
+ * and written into block_tables[b, ceil(o/T) ...]; every other entry keeps its
+ * value.  slots[t] is the slot of the step's token t, or -1: behind the last
+ * request's tokens, past the table's width, and where the free list gave no
+ * block (the table entry is then -1).  *free_used_out = *free_used + the
+ * blocks needed, which exceeds free_count when the list was too short.
+ *
+ * block_tables: [B, table_width] int32, in and out; context_lens, query_lens:
+ * [B]; query_starts: [B+1]; slots: [total_tokens] int64.  B <= 4096.
+ * context_lens_out may be context_lens and free_used_out may be free_used; the
+ * other arrays must not overlap.
+ */
+int kf_paged_block_tables(int32_t* block_tables, const int32_t* context_lens, const int32_t* query_lens,
+                          const int32_t* free_blocks, const int32_t* free_used, int32_t* query_starts,
+                          int32_t* context_lens_out, int64_t* slots, int32_t* free_used_out, int64_t B,
+                          int64_t table_width, int64_t free_count, int64_t total_tokens, int64_t block_tokens,
+                          kf_stream_t stream);
+
+/*
+ * Write the keys and values of `tokens` tokens into their slots.  For each
+ * block and head that gets tokens, a = max|x| over the new ones and
+ *   scale = max(old scale, least power of two s >= 2^-126 with a <= M s)
+ * (M = 448 or 127), code = round(clamp(x / scale, -M, M)), ties to even; codes
+ * that the block keeps are multiplied by old scale / scale and rounded.  A call
+ * that writes a block's first slot starts the block: its old scale and codes
+ * are dropped and the slots the call does not write become 0.  Where a new
+ * element is infinite or NaN the scale becomes NaN, and the attention over the
+ * block gives NaN, until the block is started again.
+ *
+ * key, value: [tokens, Hkv, D] of `dtype` (f16 or bf16) with the given strides
+ * in elements (multiples of 8; the dim is contiguous, 16-byte aligned).
+ * Slots outside the cache are skipped.  The tokens of one block must follow
+ * one another in the call, as the tokens of one request do (of two that name
+ * one slot the later is kept); else the codes of that block are unspecified.
+ */
+int kf_paged_cache_append(const void* key, const void* value, const int64_t* slots, void* key_cache,
+                          void* value_cache, float* key_scale, float* value_scale, int64_t tokens, int64_t blocks,
+                          int64_t Hkv, int64_t D, int64_t block_tokens, int64_t key_token_stride,
+                          int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride, int dtype,
+                          int cache_dtype, kf_stream_t stream);
+
+/* Workspace bytes kf_paged_attention needs (0: none) on the current device. */
+int64_t kf_paged_attention_workspace_bytes(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t max_query_len, int64_t max_context_len);
+
+/*
+ * Attention of new tokens over the cache.  Request b's queries are the tokens
+ * query_starts[b] .. query_starts[b+1]-1 of q (query_starts NULL: token b
+ * alone, tokens = B); they stand at the end of its context_lens[b] cached
+ * tokens.  Query i of n sees the keys before context - n + i + 1 (causal) or
+ * all of them:
+ *   s_j = scale * key_scale * <q, key code_j>,  lse = log sum exp(s_j),
+ *   out = sum_j exp(s_j - lse) * value_scale * value code_j.
+ * A row that sees no key gives out = 0 and lse = +inf.  A row that sees a key
+ * of a table entry outside the cache, or a key past the table's width, gives
+ * NaN.  Codes must be finite where they are read (kf_paged_cache_append writes
+ * no others); what lies behind a request's context is not looked at.
+ *
+ * q: [tokens, Hq, D] of dtype (f16 or bf16), strides in elements (multiples of
+ * 8), 16-byte aligned rows; out: [tokens, Hq, D] contiguous; lse: [Hq, tokens]
+ * or NULL.  Rows of tokens behind the last request are left as they are,
+ * except that clear_rest & 1 writes 0 into out and clear_rest & 2 +inf into
+ * lse there.  Queries of a request past max_query_len give NaN.
+ * max_context_len only guides how the keys are split over workgroups.
+ * workspace: kf_paged_attention_workspace_bytes(..) bytes (NULL where that is
+ * 0), 16-byte aligned; its contents do not matter.
+ */
+int kf_paged_attention(const void* q, const void* key_cache, const void* value_cache, const float* key_scale,
+                       const float* value_scale, const int32_t* block_tables, const int32_t* context_lens,
+                       const int32_t* query_starts, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                       int64_t tokens, int64_t B, int64_t blocks, int64_t table_width, int64_t Hq, int64_t Hkv,
+                       int64_t D, int64_t block_tokens, int64_t q_token_stride, int64_t q_head_stride,
+                       int64_t max_query_len, int64_t max_context_len, float scale, int causal, int clear_rest,
+                       int dtype, int cache_dtype, kf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ ABI_VERSION = 1
 
 KF_F32, KF_F16, KF_BF16 = 0, 1, 2
 KF_WEIGHT_NK, KF_WEIGHT_KN = 0, 1
+KF_CACHE_E4M3, KF_CACHE_INT8 = 0, 1
 TORCH_TO_KF = {torch.float32: KF_F32, torch.float16: KF_F16, torch.bfloat16: KF_BF16}
 
 _c_void_p = ctypes.c_void_p
@@ -115,6 +116,11 @@ SIGNATURES = {
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
          _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _c_void_p],
     ),
+    "kf_paged_block_tables": (_int, [_c_void_p] * 9 + [_i64] * 5 + [_c_void_p]),
+    "kf_paged_cache_append": (_int, [_c_void_p] * 7 + [_i64] * 9 + [_int, _int, _c_void_p]),
+    "kf_paged_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "kf_paged_attention": (
+        _int, [_c_void_p] * 11 + [_i64] * 13 + [_f32, _int, _int, _int, _int, _c_void_p]),
 }
 
 # Measurement kernels (kernelforge_amd/csrc/measure.hip: bench.py's copy and
@@ -148,6 +154,9 @@ MEASURE_SIGNATURES = {
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
          _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _int, _c_void_p],
     ),
+    "kfm_paged_block_of_group": (_int, [_c_void_p, _int, _int, _int, _int]),
+    "kfm_paged_block_of_slot": (_i64, [_i64, _i64, _int]),
+    "kfm_paged_request": (None, [_c_void_p, _c_void_p, _int, _int, _int, _int, _c_void_p]),
     "kfm_fa_bwd_split": (
         _int,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
