@@ -10,6 +10,8 @@
 // the largest value scale seen so far, so the product is at most 2^15 and
 // stays a normal number down to 2^-29 of the largest term (f16 rounds by at most
 // 2^-11 where bf16 would by 2^-8).  Maxima, sums and accumulators are fp32.
+#include <type_traits>
+
 #include "paged_common.h"
 
 namespace kf {
@@ -18,7 +20,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kPScale = 32768.0f;  // 2^15, the largest f16 operand of the second product
-constexpr int kMaxSplits = 64;
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
 
 struct PagedParams {
@@ -32,11 +33,9 @@ struct PagedParams {
     const int* starts;  // null: one query a request
     void* out;
     float* lse;
-    float2* ml;   // [tokens * Hq][splits]: running maximum (log2 units) and sum
-    float* part;  // [splits][tokens * Hq][D]
     int64_t q_ts, q_hs;
     int tokens, B, blocks, width, Hq, Hkv, G, D, shift;
-    int max_q, row_tiles, splits;
+    int max_q;
     float c;  // scale * log2(e)
     bool causal;
     int clear_rest;  // rows behind the last request: 1 out, 2 lse
@@ -46,388 +45,666 @@ __device__ __forceinline__ Request request(const PagedParams& p, int b) {
     return request_at(p.starts, p.context, b, p.tokens);
 }
 
+// The same for a b that is one for the wavefront: its values in scalar registers.
+__device__ __forceinline__ Request uniform_request(const PagedParams& p, int b) {
+    Request r = request(p, __builtin_amdgcn_readfirstlane(b));
+    r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
+    r.n = __builtin_amdgcn_readfirstlane(r.n);
+    r.ctx = __builtin_amdgcn_readfirstlane(r.ctx);
+    return r;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | lo);
+}
+
 __device__ __forceinline__ int reach(const PagedParams& p, const Request& r, int i) {
     return keys_seen(r, i, p.causal);
 }
 
-// The rows of tokens [from, to) of one key head, all to one value.
-// (what: 1 out, 2 lse).
+// Keys of a request to go through: one past the table at most, since that key
+// already makes the rows that see it NaN.
+__device__ __forceinline__ int keys_to_scan(const PagedParams& p, int seen) {
+    return (int)min((int64_t)seen, ((int64_t)p.width << p.shift) + 1);
+}
+
+// Every step-th token's rows of `heads` query heads, all to one value (what: 1
+// out, 2 lse).
 template <typename T>
-__device__ __forceinline__ void fill_rows(const PagedParams& p, int head, int from, int to, int what, float value,
-                                          float lse) {
+__device__ __forceinline__ void fill_rows(const PagedParams& p, int from, int to, int step, int head, int heads,
+                                          int what, float value, float lse) {
     const int vecs = p.D >> 3;
     Vec16<T> v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v.v[i] = (T)value;
-    for (int tok = from; tok < to; ++tok) {
-        const int64_t row = (int64_t)tok * p.Hq + head * p.G;
+    for (int64_t tok = from; tok < to; tok += step) {
+        const int64_t row = tok * p.Hq + head;
         if (what & 1)
-            for (int i = threadIdx.x; i < p.G * vecs; i += blockDim.x)
+            for (int64_t i = threadIdx.x; i < (int64_t)heads * vecs; i += blockDim.x)
                 *(Vec16<T>*)((T*)p.out + row * p.D + 8 * i) = v;
         if (p.lse && (what & 2))
-            for (int g = threadIdx.x; g < p.G; g += blockDim.x)
-                p.lse[(int64_t)(head * p.G + g) * p.tokens + tok] = lse;
+            for (int g = threadIdx.x; g < heads; g += blockDim.x) p.lse[(int64_t)(head + g) * p.tokens + tok] = lse;
     }
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: 16 * RT (query, head) rows of one key head per workgroup, keys
-// split over its 4 wavefronts and over workgroups.
+// Few rows: 16 * RT (query, head) rows of one key head are a unit of work, whose
+// keys the 4 wavefronts of a workgroup split.
 //
-// A wavefront takes 64 keys at a time, as four 16-token groups.  S^T = K Q^T
-// with K as the A operand: tile t's row m' is token 4t + m'%4 of group m'/4,
-// so the D layout (column = row of Q = lane%16, rows 4*(lane/16)+i) leaves lane
-// (row, quarter) with all 16 scores of its quarter's group: one key scale and
-// one value scale a lane, and exactly the B operand O^T = V^T P^T wants when
-// V^T's lane (column, quarter) holds the same 16 tokens of its column, which
-// is 16 contiguous bytes of the value cache.  Nothing passes through LDS and
-// every load is 16 bytes a lane.
+// A wavefront takes 16 * NT keys at a time.  S^T = K Q^T with K as the A
+// operand: of tile t, row m' is the key 4 NT (m'/4) + 4 t + m'%4, so the D layout
+// (column = row of Q = lane%16, rows 4*(lane/16)+i) leaves lane (row, quarter)
+// with the scores of 4 NT consecutive keys, all of one 16-token group: one key
+// scale and one value scale a lane, and exactly the B operand that
+// O^T = V^T P^T wants when V^T's lane (column, quarter) holds the same tokens
+// of its column, which are contiguous bytes of the value cache.  Nothing passes
+// through LDS before a unit's end, and every load is 16 (NT = 2: 8 for values)
+// bytes a lane.
+//
+// Bound by HBM, so the loop is built around the loads in flight: a wavefront
+// asks for the next turn's keys as soon as the products have used the
+// registers, for its values likewise, for its table entries a turn earlier, and
+// goes on to its next unit's without a pause.  Measured: 32 requests of 8192
+// keys, 8 key heads of 128 in e4m3 (537 MB), 106 us with the join, 5.1 TB/s,
+// two requests of 100001 and 60000 keys (401 MB) 82 us, 4.9 TB/s; a pass costs 12 us
+// besides 5.9 TB/s (starting, the last units, the join).
 // ---------------------------------------------------------------------------
-template <typename T, int CT, int DP, int RT>
-__global__ __launch_bounds__(256, DP * RT > 128 ? 1 : 2) void paged_rows_kernel(PagedParams p) {
-    constexpr int KC = DP / 64;   // 64-column chunks of a key row
-    constexpr int VT = DP / 16;   // 16-column tiles of the output
-    constexpr int OC = DP < 128 ? DP : 128;  // columns joined at a time
-    constexpr int PITCH = OC + 4;
-    __shared__ float s_acc[4][16][PITCH];
-    __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
+template <int DP, int RT> struct RowsShape {
+    // 16-key tiles of a turn: what two wavefronts a SIMD have registers for.
+        static constexpr int NT = DP * RT > 128 ? 2 : 4;
+    static constexpr int KEYS = 16 * NT;            // keys a wavefront takes in a turn
+    static constexpr int ROWS = 16 * RT;            // rows of a unit
+    static constexpr int OC = DP < 128 ? DP : 128;  // columns joined at a time
+};
 
+// The work is a line of turns: for each request its units (row tile, key head),
+// for each unit its keys in turns.  Every workgroup takes an equal share of the
+// line, one round of workgroups for the GPU.  The device alone knows the
+// lengths, so every workgroup sums the requests' turns for itself.  Requests of
+// any mixture of lengths then end together.  Where the contexts are short
+// (`aligned`) the line counts units and no unit is cut, so nothing is left to
+// join.
+struct Whole {
+    int q0, n, ctx;  // request
+    int row_tile, head;
+    int parts, part;  // how many (0: there is no such unit), the first one's place
+    int unused;
+};
+struct Shares {
+    float* o;     // [2 * workgroups][ROWS][D]: partial results of a workgroup's first and last segment
+    float2* ml;   // [2 * workgroups][ROWS]: running maximum (log2 units) and sum
+    Whole* whole; // [workgroups]: the unit that begins there and does not end
+    int least;    // turns of a workgroup at least
+    bool aligned;
+};
+
+// A request's units and the steps of the line that each takes.
+template <int KEYS, int ROWS>
+__device__ __forceinline__ int2 steps_and_units(const PagedParams& p, const Request& r, bool aligned) {
+    const int keys = keys_to_scan(p, r.ctx);
+    const int rows = min(r.n, p.max_q) * p.G;
+    return make_int2(aligned ? 1 : max((keys + KEYS - 1) / KEYS, 1), (rows + ROWS - 1) / ROWS * p.Hkv);
+}
+
+// a / b for b > 0; the 64-bit division only where it is needed (0.3 us of a
+// workgroup's start each).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if ((a | b) >> 32 == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    return a / b;
+}
+
+// A workgroup's stretch of one unit.
+struct Segment {
+    int b, q0, n, ctx;  // request
+    int row_tile, head;
+    int first, last;  // turns
+    int part;         // where its partial result goes; -1: it is the whole unit
+    int unit;
+};
+constexpr int kSegments = 64;  // of a workgroup at a time
+
+template <int DP, int RT> struct RowsShared {
+    float acc[4][16][RowsShape<DP, RT>::OC + 4];
+    float m[4][16 * RT], l[4][16 * RT];
+    Segment list[kSegments];
+    int64_t sum[4], units[4];
+    int64_t unit0, unit1, behind;  // global indexes of the share's first and last unit; the line behind the list
+    Whole whole;
+};
+
+// Exclusive prefix sums over the workgroup's 4 wavefronts; *total their sum.
+__device__ __forceinline__ int64_t prefix_of(int64_t mine, int64_t* scratch, int64_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t other = __shfl_up((long long)incl, off, 64);
+        if (lane >= off) incl += other;
+    }
+    if (lane == 63) scratch[wave] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, all = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k < wave) before += scratch[k];
+        all += scratch[k];
+    }
+    *total = uniform64(all);
+    return before;
+}
+
+template <typename T, int CT, int DP, int RT, bool EXACT>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Shares w) {
+    using Shape = RowsShape<DP, RT>;
+    constexpr int NT = Shape::NT, KEYS = Shape::KEYS, ROWS = Shape::ROWS, OC = Shape::OC;
+    constexpr int KC = DP / 64;  // 64-column chunks of a key row
+    constexpr int VT = DP / 16;  // 16-column tiles of the output
+    constexpr int PC = NT / 2;   // 32-key products of a turn
+    __shared__ RowsShared<DP, RT> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, quarter = lane >> 4;
-    const int b = blockIdx.x / p.row_tiles, tile_of_rows = blockIdx.x % p.row_tiles;
-    const int head = blockIdx.y, split = blockIdx.z;
-    const Request r = request(p, b);
-    const int D = p.D;
+    const int D = EXACT ? DP : p.D;
 
-    if (split == 0 && tile_of_rows == 0 && p.starts) {
-        if (r.n > p.max_q)
-            fill_rows<T>(p, head, r.q0 + p.max_q, r.q0 + r.n, 3, __builtin_nanf(""), __builtin_nanf(""));
-        if (b == p.B - 1) fill_rows<T>(p, head, r.q0 + r.n, p.tokens, p.clear_rest, 0.0f, __builtin_inff());
+    // This workgroup's share of the line.
+    const int per = (p.B + 255) / 256;
+    const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+    // A thread's first request, most often its only one, stays in registers.
+    const Request r0 = request(p, min(b0, p.B - 1));
+    auto my_request = [&](int b) { return b == b0 ? r0 : request(p, b); };
+    int64_t my_steps = 0, my_units = 0, total, all_units;
+    for (int b = b0; b < b1; ++b) {
+        const int2 su = steps_and_units<KEYS, ROWS>(p, my_request(b), w.aligned);
+        my_steps += (int64_t)su.x * su.y;
+        my_units += su.y;
     }
-    const int row0 = tile_of_rows * 16 * RT, rows = min(r.n, p.max_q) * p.G;
-    if (row0 >= rows) return;
+    const int64_t steps_before = prefix_of(my_steps, sh.sum, &total);
+    const int64_t units_before = prefix_of(my_units, sh.units, &all_units);
+    const int64_t share = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)w.least);
+    const int64_t begin = blockIdx.x * share, end = min(begin + share, total);
+    if (p.starts) {  // tokens behind the last request
+        const Request r = request(p, p.B - 1);
+        fill_rows<T>(p, r.q0 + r.n + blockIdx.x, p.tokens, gridDim.x, 0, p.Hq, p.clear_rest, 0.0f, __builtin_inff());
+    }
+    if (tid == 0) sh.whole.parts = 0;
 
-    // This lane's rows (columns of S^T).
-    int limit[RT];
+    const int subs = (1 << (p.shift - 4)) - 1;   // groups of a block - 1
+    const int64_t unit_bytes = (int64_t)D << p.shift;  // a block's keys of one head
+    const int kgroup = 4 * NT * (m >> 2), vgroup = 4 * NT * quarter;  // first key of this lane's in a turn
     typename V<T>::x8 qf[RT][KC][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = row0 + 16 * rt + m, i = row / p.G;
-        const bool live = row < rows;
-        limit[rt] = live ? reach(p, r, i) : 0;
-        const T* q = (const T*)p.q + (int64_t)(r.q0 + i) * p.q_ts + (int64_t)(head * p.G + row % p.G) * p.q_hs;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int col = 64 * c + 16 * quarter + 8 * h;
-                u32x4 v = {0u, 0u, 0u, 0u};
-                if (live && col < D) v = *(const u32x4*)(q + col);
-                qf[rt][c][h] = __builtin_bit_cast(typename V<T>::x8, v);
-            }
-    }
-    // Keys that every row sees, and that any row sees (one past the table at
-    // most: that key already makes the row NaN).
-    const int all_see = reach(p, r, row0 / p.G);
-    const int64_t table_keys = ((int64_t)p.width << p.shift) + 1;
-    const int any_sees = (int)min((int64_t)reach(p, r, (min(row0 + 16 * RT, rows) - 1) / p.G), table_keys);
-    const int tiles = (any_sees + 63) >> 6;
-    const int per_split = (tiles + p.splits - 1) / p.splits;
-    const int first = split * per_split, last = min(first + per_split, tiles);
-    const int per_wave = max((last - first + 3) / 4, 0);
-    const int t0 = first + wave * per_wave, t1 = min(t0 + per_wave, last);
-
-    const int* table = p.tables + (int64_t)b * p.width;
-    const int subs = (1 << (p.shift - 4)) - 1;  // groups of a block - 1
-    const int64_t unit = (int64_t)D << p.shift;  // bytes of a block's keys of one head
-    auto id_of = [&](int group) { return block_of_group(table, p.width, p.blocks, p.shift, group); };
-    u32x4 kr[4][KC], vr[VT];
-    auto load_keys = [&](int tile, int id) {
-        const int sub = (4 * tile + (m >> 2)) & subs;
-        const uint8_t* base = p.kc + ((int64_t)max(id, 0) * p.Hkv + head) * unit + (16 * sub + (m & 3)) * D;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const int col = 64 * c + 16 * quarter;  // past D: any bytes, the query is 0 there
-                kr[t][c] = *(const u32x4*)(base + 4 * t * D + (col < D ? col : 0));
-            }
-    };
-    auto load_values = [&](int tile, int id) {
-        const int sub = (4 * tile + quarter) & subs;
-        const uint8_t* base = p.vc + ((int64_t)max(id, 0) * p.Hkv + head) * unit + 16 * sub * D;
-#pragma unroll
-        for (int d = 0; d < VT; ++d)
-            if (16 * d < D) vr[d] = *(const u32x4*)(base + (16 * d + m) * 16);
-    };
-
-    f32x4 acc[RT][VT];
-    float top[RT], sum[RT], vref = kLeastScale, inv_vref = 1.0f / kLeastScale;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        top[rt] = -__builtin_inff();
-        sum[rt] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < VT; ++d) acc[rt][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    int idk = -1, idv = -1, next_idk = -1, next_idv = -1;
+    u32x4 kr[NT][KC];
+    uint32_t vr[VT][NT];
     float ks = 0.0f, vs = 0.0f;
-    auto load_scales = [&](int id) {
-        const int64_t at = (int64_t)max(id, 0) * p.Hkv + head;
-        ks = p.ks[at];
-        vs = p.vs[at];
-    };
-    if (t0 < t1) {
-        idk = id_of(4 * t0 + (m >> 2));
-        idv = id_of(4 * t0 + quarter);
-        load_scales(idv);
-        load_keys(t0, idk);
-        load_values(t0, idv);
-        if (t0 + 1 < t1) {
-            next_idk = id_of(4 * t0 + 4 + (m >> 2));
-            next_idv = id_of(4 * t0 + 4 + quarter);
-        }
-    }
-    for (int tile = t0; tile < t1; ++tile) {
-        f32x4 s[RT][4];
+    auto load_queries = [&](const Segment& g) {
+        const int rows = min(g.n, p.max_q) * p.G;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rt = 0; rt < RT; ++rt) {
+            const int row = g.row_tile * ROWS + 16 * rt + m, i = row / p.G;
+            const T* q = (const T*)p.q + (int64_t)(g.q0 + i) * p.q_ts + (int64_t)(g.head * p.G + row % p.G) * p.q_hs;
 #pragma unroll
             for (int c = 0; c < KC; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const auto a = Codes<T, CT>::x8(kr[t][c][2 * h], kr[t][c][2 * h + 1]);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c][h], s[rt][t]);
+                    const int col = 64 * c + 16 * quarter + 8 * h;
+                    u32x4 v = {0u, 0u, 0u, 0u};
+                    if (row < rows && col < D) v = *(const u32x4*)(q + col);
+                    qf[rt][c][h] = __builtin_bit_cast(typename V<T>::x8, v);
                 }
         }
-        const int group0 = tile * 64 + 16 * quarter;  // position of this lane's first key
-        const bool bad = idv < 0 && group0 < r.ctx;
-        const bool edge = tile * 64 + 64 > all_see || __any(idv < 0);
-        const float kscale = bad ? __builtin_nanf("") : ks * p.c;
-        // Blocks behind the context say nothing; an infinite scale is a NaN, which
-        // only the rows that see its block take on.
-        const float vscale = idv < 0 || group0 >= r.ctx ? 0.0f : vs < __builtin_inff() ? vs : __builtin_nanf("");
-        const int idv_now = idv;
-        if (tile + 1 < t1) {
-            idk = next_idk;
-            idv = next_idv;
-            load_scales(idv);
-            load_keys(tile + 1, idk);
-            if (tile + 2 < t1) {
-                next_idk = id_of(4 * tile + 8 + (m >> 2));
-                next_idv = id_of(4 * tile + 8 + quarter);
+    };
+    // A table entry is looked at only when its turn comes: a check right behind its
+    // load would wait for every load issued before it, the next keys among them.
+    auto entry_of = [&](int b, int key) {
+        return entry_of_group(p.tables + (int64_t)b * p.width, p.width, p.shift, key >> 4);
+    };
+    auto block_of = [&](int id, int key) { return block_of_entry(id, p.width, p.blocks, p.shift, key >> 4); };
+    auto load_keys = [&](int head, int turn, int idk, int idv) {
+        const int64_t at = (int64_t)max(idv, 0) * p.Hkv + head;
+        ks = p.ks[at];
+        vs = p.vs[at];
+        __builtin_amdgcn_sched_barrier(0);
+        const int key = KEYS * turn + kgroup;
+        const uint8_t* from = p.kc + ((int64_t)max(idk, 0) * p.Hkv + head) * unit_bytes +
+                              (16 * ((key >> 4) & subs) + (key & 15) + (m & 3)) * D;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const int col = 64 * c + 16 * quarter;  // past D: any bytes, the query is 0 there
+                kr[t][c] = *(const u32x4*)(from + 4 * t * D + (col < D ? col : 0));
+                __builtin_amdgcn_sched_barrier(0);
             }
+    };
+    auto load_values = [&](int head, int turn, int id) {
+        const int key = KEYS * turn + vgroup;
+        const uint8_t* from =
+            p.vc + ((int64_t)max(id, 0) * p.Hkv + head) * unit_bytes + 16 * ((key >> 4) & subs) * D + (key & 15);
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+            const int col = 16 * d < D ? 16 * d : 0;  // past D: columns that are not written
+            if constexpr (NT == 4) {
+                const u32x4 v = *(const u32x4*)(from + (col + m) * 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) vr[d][k] = v[k];
+            } else {
+                const u32x2 v = *(const u32x2*)(from + (col + m) * 16);
+                vr[d][0] = v[0];
+                vr[d][1] = v[1];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
 
-        // The largest value scale so far, the same on every lane.
-        float vmax = fmaxf(vscale, __shfl_xor(vscale, 16, 64));
-        vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
-        float shrink = 1.0f;
-        if (vmax > vref) {
-            shrink = vref / vmax;
-            vref = vmax;
-            inv_vref = 1.0f / vmax;
-        }
-        const float factor = vscale * inv_vref * kPScale;
+    auto segment_at = [&](int k) {
+        Segment g = sh.list[k];
+        int* x = (int*)&g;
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(Segment) / 4); ++e) x[e] = __builtin_amdgcn_readfirstlane(x[e]);
+        return g;
+    };
+    // This wavefront's turns of a segment: a quarter of them.  One without a turn
+    // of its own goes through the first with every key hidden.
+    auto turns_of = [&](const Segment& g) {
+        const int per_wave = (g.last - g.first + 3) >> 2, t0 = g.first + wave * per_wave;
+        return t0 < g.last ? make_int2(t0, min(t0 + per_wave, g.last)) : make_int2(g.first, g.first + 1);
+    };
 
-        V<f16>::x8 pf[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float most = -__builtin_inff();
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = s[rt][t][i] * kscale;
-                    if (edge && group0 + 4 * t + i >= limit[rt]) x = -__builtin_inff();
-                    s[rt][t][i] = x;
-                    most = fmaxf(most, x);
-                }
-            most = fmaxf(most, __shfl_xor(most, 16, 64));
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
-            const float now = fmaxf(top[rt], most);
-            const float base = now == -__builtin_inff() ? 0.0f : now;
-            const float alpha = __builtin_amdgcn_exp2f(top[rt] - base);
-            top[rt] = now;
-            float add = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - base);
-                    add += e;
-                    // A hidden key's weight is 0 whatever its block's scale.
-                    const float w = edge && group0 + 4 * t + i >= limit[rt] ? 0.0f : e * factor;
-                    pf[rt][t >> 1][4 * (t & 1) + i] = (f16)w;
-                }
-            sum[rt] = sum[rt] * alpha + add;
-            const float keep = alpha * shrink;
-            if (__any(keep != 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < VT; ++d) acc[rt][d] *= keep;
+    for (int64_t from = begin; from < end;) {
+        // The next segments of the share, in order.
+        __syncthreads();
+        {
+            int64_t base = steps_before, unit_base = units_before;
+            for (int b = b0; b < b1; ++b) {
+                const int2 su = steps_and_units<KEYS, ROWS>(p, my_request(b), w.aligned);
+                const int64_t after = base + (int64_t)su.x * su.y;
+                if (from >= base && from < after) sh.unit0 = unit_base + quotient(from - base, su.x);
+                if (end - 1 >= base && end - 1 < after) sh.unit1 = unit_base + quotient(end - 1 - base, su.x);
+                base = after;
+                unit_base += su.y;
             }
         }
-        if (edge) {
-            // Codes behind the context or of no block are not looked at.
-            const int valid = idv_now < 0 ? 0 : min(max(r.ctx - group0, 0), 16);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int bytes = min(max(valid - 4 * k, 0), 4);
-                const uint32_t mask = bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1u;
-#pragma unroll
-                for (int d = 0; d < VT; ++d) vr[d][k] &= mask;
+        __syncthreads();
+        const int64_t unit0 = uniform64(sh.unit0), unit1 = uniform64(sh.unit1);
+        const int count = (int)min(unit1 - unit0 + 1, (int64_t)kSegments);
+        {
+            int64_t base = steps_before, unit_base = units_before;
+            for (int b = b0; b < b1; ++b) {
+                const Request r = my_request(b);
+                const int2 su = steps_and_units<KEYS, ROWS>(p, r, w.aligned);
+                const int u0 = (int)min(max(unit0 - unit_base, (int64_t)0), (int64_t)su.y);
+                const int u1 = (int)max(min(unit0 + count - unit_base, (int64_t)su.y), (int64_t)0);
+                for (int u = u0; u < u1; ++u) {
+                    const int64_t unit_begin = base + (int64_t)u * su.x, unit_end = unit_begin + su.x;
+                    const int64_t x = max(from, unit_begin), y = min(end, unit_end);
+                    Segment g;
+                    g.b = b;
+                    g.q0 = r.q0;
+                    g.n = r.n;
+                    g.ctx = r.ctx;
+                    g.unit = u;
+                    g.row_tile = u / p.Hkv;
+                    g.head = u - g.row_tile * p.Hkv;
+                    const int rows = min(r.n, p.max_q) * p.G;
+                    const int sees = keys_to_scan(p, reach(p, r, (min((g.row_tile + 1) * ROWS, rows) - 1) / p.G));
+                    const int turns = (sees + KEYS - 1) / KEYS;
+                    g.first = w.aligned ? 0 : (int)(x - unit_begin);
+                    g.last = w.aligned ? turns : min((int)(y - unit_begin), turns);
+                    g.part = -1;
+                    if (y - x != su.x) {
+                        g.part = 2 * blockIdx.x + (x == begin ? 0 : 1);
+                        if (x == unit_begin)
+                            sh.whole = Whole{r.q0, r.n, r.ctx, g.row_tile, g.head,
+                                             (int)quotient(unit_end - 1, share) - (int)blockIdx.x + 1, g.part, 0};
+                    }
+                    const int at = (int)(unit_base + u - unit0);
+                    sh.list[at] = g;
+                    if (at == count - 1) sh.behind = y;
+                }
+                base += (int64_t)su.x * su.y;
+                unit_base += su.y;
             }
         }
+        __syncthreads();
+        from = uniform64(sh.behind);
+
+        // The registers hold the keys and values of (cur, turn); next_id* are the
+        // table entries of the turn behind it, of this segment or of the next.  The
+        // loads of a turn are issued in one order everywhere (scales, keys, entries,
+        // values) and whether or not there is a turn to come (the last one's are
+        // repeated): a wait for the oldest of them then leaves the others in flight.
+        Segment cur = segment_at(0), nxt = segment_at(min(1, count - 1));
+        int2 turns = turns_of(cur), next_turns = turns_of(nxt);
+        int turn = turns.x;
+        int next_idk, next_idv;
+        auto load_entries = [&](int b, int at) {
+            next_idk = entry_of(b, KEYS * at + kgroup);
+            next_idv = entry_of(b, KEYS * at + vgroup);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        load_entries(cur.b, turn);
+        load_queries(cur);
+        int idk = block_of(next_idk, KEYS * turn + kgroup), idv = block_of(next_idv, KEYS * turn + vgroup);
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys(cur.head, turn, idk, idv);
+        load_entries(turn + 1 < turns.y ? cur.b : nxt.b, turn + 1 < turns.y ? turn + 1 : next_turns.x);
+        load_values(cur.head, turn, idv);
+        for (int k = 0; k < count; ++k) {
+            const Request r{cur.q0, cur.n, cur.ctx};
+            const Segment later = segment_at(min(k + 2, count - 1));
+            const int2 later_turns = turns_of(later);
+            const int row0 = cur.row_tile * ROWS, rows = min(r.n, p.max_q) * p.G;
+            if (cur.row_tile == 0 && cur.first == 0 && r.n > p.max_q)
+                fill_rows<T>(p, r.q0 + p.max_q, r.q0 + r.n, 1, cur.head * p.G, p.G, 3, __builtin_nanf(""),
+                             __builtin_nanf(""));
+            // This lane's rows (columns of S^T).
+            const bool idle = cur.first + wave * ((cur.last - cur.first + 3) >> 2) >= cur.last;
+            int limit[RT];
+            f32x4 acc[RT][VT];
+            float top[RT], sum[RT], vref = kLeastScale, inv_vref = 1.0f / kLeastScale;
 #pragma unroll
-        for (int d = 0; d < VT; ++d)
-            if (16 * d < D) {
+            for (int rt = 0; rt < RT; ++rt) {
+                const int row = row0 + 16 * rt + m;
+                limit[rt] = row < rows && !idle ? reach(p, r, row / p.G) : 0;
+                top[rt] = -__builtin_inff();
+                sum[rt] = 0.0f;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const auto a = Codes<f16, CT>::x8(vr[d][2 * h], vr[d][2 * h + 1]);
+                for (int d = 0; d < VT; ++d) acc[rt][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            const int all_see = idle ? 0 : reach(p, r, row0 / p.G);  // keys that every row sees
+
+            for (; turn < turns.y; ++turn) {
+                f32x4 s[RT][NT];
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const auto a = Codes<T, CT>::x8(kr[t][c][2 * h], kr[t][c][2 * h + 1]);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c][h], s[rt][t]);
+                        }
+                }
+                const int key0 = turn * KEYS + vgroup;  // position of this lane's first key
+                const bool bad = idv < 0 && key0 < r.ctx;
+                const bool edge = turn * KEYS + KEYS > all_see || __any(idv < 0);
+                const float kscale = bad ? __builtin_nanf("") : ks * p.c;
+                // Blocks behind the context say nothing; an infinite scale is a NaN, which
+                // only the rows that see its block take on.
+                const float vscale = idv < 0 || key0 >= r.ctx ? 0.0f : vs < __builtin_inff() ? vs : __builtin_nanf("");
+                const int idv_now = idv;
+                const bool same = turn + 1 < turns.y;
+                const int then = same ? turn + 1 : next_turns.x, then_head = same ? cur.head : nxt.head;
+                idk = block_of(next_idk, KEYS * then + kgroup);
+                idv = block_of(next_idv, KEYS * then + vgroup);
+                if (!same) load_queries(nxt);
+                load_keys(then_head, then, idk, idv);
+                {
+                    const bool inside = turn + 2 < turns.y, behind = next_turns.x + 1 < next_turns.y;
+                    load_entries(inside ? cur.b : same || behind ? nxt.b : later.b,
+                                 inside ? turn + 2 : same ? next_turns.x : behind ? next_turns.x + 1 : later_turns.x);
+                }
+
+                // The largest value scale so far, the same on every lane.
+                float vmax = fmaxf(vscale, __shfl_xor(vscale, 16, 64));
+                vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
+                float shrink = 1.0f;
+                if (vmax > vref) {
+                    shrink = vref / vmax;
+                    vref = vmax;
+                    inv_vref = 1.0f / vmax;
+                }
+                const float factor = vscale * inv_vref * kPScale;
+
+                V<f16>::x8 pf[RT][PC];
+                auto softmax = [&](auto at_edge) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float most = -__builtin_inff();
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float x = s[rt][t][i] * kscale;
+                                if (decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt]) x = -__builtin_inff();
+                                s[rt][t][i] = x;
+                                most = fmaxf(most, x);
+                            }
+                        most = fmaxf(most, __shfl_xor(most, 16, 64));
+                        most = fmaxf(most, __shfl_xor(most, 32, 64));
+                        const float now = fmaxf(top[rt], most);
+                        const float ref = now == -__builtin_inff() ? 0.0f : now;
+                        const float alpha = __builtin_amdgcn_exp2f(top[rt] - ref);
+                        top[rt] = now;
+                        float add = 0.0f;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - ref);
+                                add += e;
+                                // A hidden key's weight is 0 whatever its block's scale.
+                                const float x =
+                                    decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt] ? 0.0f : e * factor;
+                                pf[rt][t >> 1][4 * (t & 1) + i] = (f16)x;
+                            }
+                        sum[rt] = sum[rt] * alpha + add;
+                        const float keep = alpha * shrink;
+                        // Always: a way around the products would keep two copies of them.
+#pragma unroll
+                        for (int d = 0; d < VT; ++d) acc[rt][d] *= keep;
+                    }
+                };
+                if (edge)
+                    softmax(std::true_type());
+                else
+                    softmax(std::false_type());
+                // Codes behind the context or of no block are not looked at.
+                const int valid = idv_now < 0 ? 0 : min(max(r.ctx - key0, 0), 4 * NT);
+                uint32_t mask[NT];
+#pragma unroll
+                for (int e = 0; e < NT; ++e) {
+                    const int bytes = min(max(valid - 4 * e, 0), 4);
+                    mask[e] = bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1u;
+                }
+#pragma unroll
+                for (int d = 0; d < VT; ++d)
+#pragma unroll
+                    for (int h = 0; h < PC; ++h) {
+                        const auto a = Codes<f16, CT>::x8(vr[d][2 * h] & mask[2 * h], vr[d][2 * h + 1] & mask[2 * h + 1]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
+                    }
+                load_values(then_head, then, idv);
+            }
+
+            // Join the four wavefronts, 16 rows and OC columns at a time.
+            __syncthreads();  // the segment before has read its sums
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                sum[rt] += __shfl_xor(sum[rt], 16, 64);
+                sum[rt] += __shfl_xor(sum[rt], 32, 64);
+                if (quarter == 0) {
+                    sh.m[wave][16 * rt + m] = top[rt];
+                    sh.l[wave][16 * rt + m] = sum[rt];
                 }
             }
-        if (tile + 1 < t1) load_values(tile + 1, idv);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int d0 = 0; d0 < DP; d0 += OC) {
+                    if (rt + d0 > 0) __syncthreads();
+#pragma unroll
+                    for (int d = 0; d < OC / 16; ++d)
+                        *(f32x4*)&sh.acc[wave][m][16 * d + 4 * quarter] = acc[rt][d0 / 16 + d] * (1.0f / kPScale) * vref;
+                    __syncthreads();
+                    const int x = tid >> 4, col = 8 * (tid & 15);
+                    const int row = row0 + 16 * rt + x;
+                    if (row >= rows || col >= OC || d0 + col >= D) continue;
+                    float best = sh.m[0][16 * rt + x];
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) best = fmaxf(best, sh.m[k][16 * rt + x]);
+                    const float ref = best == -__builtin_inff() ? 0.0f : best;
+                    float l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float lk = sh.l[k][16 * rt + x];
+                        if (lk == 0.0f) continue;
+                        const float f = __builtin_amdgcn_exp2f(sh.m[k][16 * rt + x] - ref);
+                        l += f * lk;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] += f * sh.acc[k][x][col + e];
+                    }
+                    if (cur.part >= 0) {
+                        const int64_t at = (int64_t)cur.part * ROWS + 16 * rt + x;
+                        if (d0 == 0 && col == 0) w.ml[at] = make_float2(best, l);
+                        float* to = w.o + at * D + d0 + col;
+                        *(f32x4*)to = (f32x4){o[0], o[1], o[2], o[3]};
+                        *(f32x4*)(to + 4) = (f32x4){o[4], o[5], o[6], o[7]};
+                        continue;
+                    }
+                    const int i = row / p.G;
+                    const int64_t at = (int64_t)(r.q0 + i) * p.Hq + cur.head * p.G + row % p.G;
+                    const bool none = reach(p, r, i) <= 0;
+                    Vec16<T> v;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v.v[e] = (T)(none ? 0.0f : o[e] / l);
+                    *(Vec16<T>*)((T*)p.out + at * D + d0 + col) = v;
+                    if (p.lse && d0 == 0 && col == 0)
+                        p.lse[(int64_t)(cur.head * p.G + row % p.G) * p.tokens + r.q0 + i] =
+                            none ? __builtin_inff() : (best + log2f(l)) * kLn2;
+                }
+            cur = nxt;
+            nxt = later;
+            turns = next_turns;
+            next_turns = later_turns;
+            turn = turns.x;
+        }
     }
-
-    // Join the four wavefronts, 16 rows and OC columns at a time.
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        sum[rt] += __shfl_xor(sum[rt], 16, 64);
-        sum[rt] += __shfl_xor(sum[rt], 32, 64);
-        if (quarter == 0) {
-            s_m[wave][16 * rt + m] = top[rt];
-            s_l[wave][16 * rt + m] = sum[rt];
-        }
+    if (!w.aligned) {
+        __syncthreads();
+        if (tid == 0) w.whole[blockIdx.x] = sh.whole;
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int d0 = 0; d0 < DP; d0 += OC) {
-            __syncthreads();
-#pragma unroll
-            for (int d = 0; d < OC / 16; ++d)
-                *(f32x4*)&s_acc[wave][m][16 * d + 4 * quarter] =
-                    acc[rt][d0 / 16 + d] * (1.0f / kPScale) * vref;
-            __syncthreads();
-            const int x = threadIdx.x >> 4, col = 8 * (threadIdx.x & 15);
-            const int row = row0 + 16 * rt + x;
-            if (row >= rows || col >= OC || d0 + col >= D) continue;
-            float best = s_m[0][16 * rt + x];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) best = fmaxf(best, s_m[w][16 * rt + x]);
-            float l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float lw = s_l[w][16 * rt + x];
-                if (lw == 0.0f) continue;
-                const float f = __builtin_amdgcn_exp2f(s_m[w][16 * rt + x] - best);
-                l += f * lw;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] += f * s_acc[w][x][col + k];
-            }
-            const int i = row / p.G;
-            const int64_t at = (int64_t)(r.q0 + i) * p.Hq + head * p.G + row % p.G;
-            if (p.splits > 1) {
-                if (d0 == 0 && col == 0) p.ml[at * p.splits + split] = make_float2(best, l);
-                if (l != 0.0f) {
-                    float* to = p.part + ((int64_t)split * p.tokens * p.Hq + at) * D + d0 + col;
-                    *(f32x4*)to = (f32x4){o[0], o[1], o[2], o[3]};
-                    *(f32x4*)(to + 4) = (f32x4){o[4], o[5], o[6], o[7]};
-                }
-                continue;
-            }
-            const bool none = reach(p, r, i) <= 0;
-            Vec16<T> v;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v.v[k] = (T)(none ? 0.0f : o[k] / l);
-            *(Vec16<T>*)((T*)p.out + at * D + d0 + col) = v;
-            if (p.lse && d0 == 0 && col == 0)
-                p.lse[(int64_t)(head * p.G + row % p.G) * p.tokens + r.q0 + i] =
-                    none ? __builtin_inff() : (best + log2f(l)) * kLn2;
-        }
 }
 
-// Joins the splits' partial results in order: 16 rows of one key head per
-// workgroup, 8 columns a thread.
-template <typename T> __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, int tiles16) {
-    const int b = blockIdx.x / tiles16, head = blockIdx.y;
-    const Request r = request(p, b);
-    const int rows = min(r.n, p.max_q) * p.G;
-    const int row = (blockIdx.x % tiles16) * 16 + (threadIdx.x >> 4);
-    if (row >= rows) return;
-    const int i = row / p.G;
-    const int64_t at = (int64_t)(r.q0 + i) * p.Hq + head * p.G + row % p.G;
-    const float2* ml = p.ml + at * p.splits;
-    float best = -__builtin_inff();
-    for (int s = 0; s < p.splits; ++s) best = fmaxf(best, ml[s].x);
-    const bool none = reach(p, r, i) <= 0;
-    for (int col = 8 * (threadIdx.x & 15); col < p.D; col += 128) {
-        float l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < p.splits; ++s) {
-            const float2 one = ml[s];
-            if (one.y == 0.0f) continue;
-            const float f = __builtin_amdgcn_exp2f(one.x - best);
-            l += f * one.y;
-            const float* from = p.part + ((int64_t)s * p.tokens * p.Hq + at) * p.D + col;
-            const f32x4 x = *(const f32x4*)from, y = *(const f32x4*)(from + 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k] += f * x[k];
-                o[4 + k] += f * y[k];
-            }
+// Joins the parts of the unit that begins in workgroup blockIdx.x's share: its
+// own part and the first part of each workgroup behind it.  LANES threads hold a
+// row's columns, eight each, and WAYS sets of them take every WAYS-th part; the
+// sets meet in LDS.  The order of the additions follows from the lengths alone.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, Shares w, int unit_rows) {
+    constexpr int WAYS = 128 / LANES;  // two rows a workgroup
+    __shared__ f32x4 s_o[2][256];
+    __shared__ float2 s_ml[256];
+    const Whole whole = w.whole[blockIdx.x];
+    const int parts = whole.parts;
+    if (parts == 0) return;
+    const int tid = threadIdx.x, col = 8 * (tid % LANES), way = tid / LANES % WAYS;
+    const int x = blockIdx.y * 2 + tid / 128;  // row of the unit
+    const Request r{whole.q0, whole.n, whole.ctx};
+    const int head = whole.head, row = whole.row_tile * unit_rows + x;
+    const bool live = row < min(r.n, p.max_q) * p.G && col < p.D;
+    float m = -__builtin_inff(), l = 0.0f;
+    f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0;
+    if (live) {
+#pragma unroll 8
+        for (int k = way; k < parts; k += WAYS) {
+            const int64_t at = (int64_t)(k == 0 ? whole.part : 2 * ((int)blockIdx.x + k)) * unit_rows + x;
+            const float2 one = w.ml[at];
+            const f32x4 y0 = *(const f32x4*)(w.o + at * p.D + col), y1 = *(const f32x4*)(w.o + at * p.D + col + 4);
+            const float now = fmaxf(m, one.x);
+            const float base = now == -__builtin_inff() ? 0.0f : now;
+            const float a = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(one.x - base);
+            l = l * a + one.y * f;
+            o0 = o0 * a + y0 * f;
+            o1 = o1 * a + y1 * f;
+            m = now;
         }
-        Vec16<T> v;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v.v[k] = (T)(none ? 0.0f : o[k] / l);
-        *(Vec16<T>*)((T*)p.out + at * p.D + col) = v;
-        if (p.lse && col == 0)
-            p.lse[(int64_t)(head * p.G + row % p.G) * p.tokens + r.q0 + i] =
-                none ? __builtin_inff() : (best + log2f(l)) * kLn2;
     }
+    s_o[0][tid] = o0;
+    s_o[1][tid] = o1;
+    s_ml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (!live || way != 0) return;
+    float best = m;
+#pragma unroll
+    for (int k = 1; k < WAYS; ++k) best = fmaxf(best, s_ml[tid + k * LANES].x);
+    const float base = best == -__builtin_inff() ? 0.0f : best;
+    l = 0.0f;
+    o0 = o1 = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < WAYS; ++k) {
+        const float2 one = s_ml[tid + k * LANES];
+        const float f = __builtin_amdgcn_exp2f(one.x - base);
+        l += one.y * f;
+        o0 += s_o[0][tid + k * LANES] * f;
+        o1 += s_o[1][tid + k * LANES] * f;
+    }
+    const int i = row / p.G, token = r.q0 + i, h = head * p.G + row % p.G;
+    const bool none = reach(p, r, i) <= 0;
+    Vec16<T> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v.v[k] = (T)(none ? 0.0f : o0[k] / l);
+        v.v[4 + k] = (T)(none ? 0.0f : o1[k] / l);
+    }
+    *(Vec16<T>*)((T*)p.out + ((int64_t)token * p.Hq + h) * p.D + col) = v;
+    if (p.lse && col == 0) p.lse[(int64_t)h * p.tokens + token] = none ? __builtin_inff() : (best + log2f(l)) * kLn2;
 }
 
 struct Plan {
-    int rt, row_tiles, splits;
-    int64_t bytes;
+    int rt;
+    bool aligned;
+    int64_t groups, bytes;
 };
 
-Plan plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
+Plan plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
     Plan r;
     const int64_t rows = max_q * (Hq / Hkv);
     r.rt = rows <= 16 || D > 128 ? 1 : 2;
-    r.row_tiles = (int)((rows + 16 * r.rt - 1) / (16 * r.rt));
-    const int64_t groups = B * r.row_tiles * Hkv;
-    const int64_t want = (4 * device_cu_count() + groups - 1) / (groups > 0 ? groups : 1);
-    const int64_t most = (max_ctx + 255) / 256;  // a tile for each wavefront
-    int64_t splits = want < most ? want : most;
-    if (splits > kMaxSplits) splits = kMaxSplits;
-    r.splits = splits > 1 ? (int)splits : 1;
-    const int64_t n = tokens * Hq * r.splits;
-    r.bytes = r.splits > 1 ? n * 8 + n * D * 4 : 0;
+    const int64_t units = B * ((rows + 16 * r.rt - 1) / (16 * r.rt)) * Hkv;
+    // A second launch joins the parts of cut units (5 us).  One workgroup takes
+    // 1024 keys in about as much.
+    r.aligned = max_ctx <= 1024;
+    // One workgroup a CU streams fastest (two requests of 100000 keys, 16 units: 82
+    // us against 86 with two, which fit); a second hides the ends of the first's
+    // units where each workgroup may have several (32 requests of 500 to 8192 keys,
+    // 256 units: 73 us against 77; 64 of 100 to 2048: 49 against 55).
+    r.groups = device_cu_count() * (units >= device_cu_count() ? 2 : 1);
+    if (r.aligned && units < r.groups) r.groups = units;
+    r.bytes = r.aligned ? 0 : r.groups * (2 * 16 * r.rt * (D * 4 + 8) + sizeof(Whole));
     return r;
 }
 
-template <typename T, int CT> void launch(const PagedParams& p, const Plan& w, hipStream_t s) {
-    const dim3 grid((unsigned)(p.B * w.row_tiles), (unsigned)p.Hkv, (unsigned)w.splits);
-    if (p.D <= 64) {
-        if (w.rt == 1)
-            paged_rows_kernel<T, CT, 64, 1><<<grid, 256, 0, s>>>(p);
-        else
-            paged_rows_kernel<T, CT, 64, 2><<<grid, 256, 0, s>>>(p);
-    } else if (p.D <= 128) {
-        if (w.rt == 1)
-            paged_rows_kernel<T, CT, 128, 1><<<grid, 256, 0, s>>>(p);
-        else
-            paged_rows_kernel<T, CT, 128, 2><<<grid, 256, 0, s>>>(p);
-    } else {
-        paged_rows_kernel<T, CT, 256, 1><<<grid, 256, 0, s>>>(p);
-    }
+template <typename T, int CT, int DP, int RT>
+void launch_rows(const PagedParams& p, const Plan& w, const Shares& sh, hipStream_t s) {
+    if (p.D == DP)
+        paged_rows_kernel<T, CT, DP, RT, true><<<dim3((unsigned)w.groups), 256, 0, s>>>(p, sh);
+    else
+        paged_rows_kernel<T, CT, DP, RT, false><<<dim3((unsigned)w.groups), 256, 0, s>>>(p, sh);
+}
+
+template <typename T, int CT> void launch(const PagedParams& p, const Plan& w, const Shares& sh, hipStream_t s) {
+    if (p.D <= 64)
+        w.rt == 1 ? launch_rows<T, CT, 64, 1>(p, w, sh, s) : launch_rows<T, CT, 64, 2>(p, w, sh, s);
+    else if (p.D <= 128)
+        w.rt == 1 ? launch_rows<T, CT, 128, 1>(p, w, sh, s) : launch_rows<T, CT, 128, 2>(p, w, sh, s);
+    else
+        launch_rows<T, CT, 256, 1>(p, w, sh, s);
+}
+
+template <typename T> void launch_join(const PagedParams& p, const Plan& w, const Shares& sh, hipStream_t s) {
+    const int unit_rows = 16 * w.rt;
+    const int64_t rows = (int64_t)p.max_q * p.G < unit_rows ? (int64_t)p.max_q * p.G : unit_rows;
+    const dim3 grid((unsigned)w.groups, (unsigned)((rows + 1) / 2));
+    if (p.D <= 64)
+        paged_join_kernel<T, 8><<<grid, 256, 0, s>>>(p, sh, unit_rows);
+    else if (p.D <= 128)
+        paged_join_kernel<T, 16><<<grid, 256, 0, s>>>(p, sh, unit_rows);
+    else
+        paged_join_kernel<T, 32><<<grid, 256, 0, s>>>(p, sh, unit_rows);
 }
 
 int check_shape(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
@@ -436,7 +713,7 @@ int check_shape(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
     KF_REQUIRE(Hq % Hkv == 0, KF_E_INVALID, "kf_paged_attention: Hq must be a multiple of Hkv");
     KF_REQUIRE(D >= 16 && D <= 256 && D % 16 == 0, KF_E_INVALID,
                "kf_paged_attention: head dim must be a multiple of 16 <= 256");
-    KF_REQUIRE(tokens <= INT32_MAX / 2 && B <= INT32_MAX / 2 && Hkv <= 65535 && Hq <= INT32_MAX / 2 &&
+    KF_REQUIRE(tokens * Hq <= INT32_MAX / 2 && B <= INT32_MAX / 2 && Hkv <= 65535 &&
                    max_q * (Hq / Hkv) <= INT32_MAX / 2 && B * ((max_q * (Hq / Hkv) + 15) / 16) <= INT32_MAX / 2,
                KF_E_UNSUPPORTED, "kf_paged_attention: too many rows");
     return KF_OK;
@@ -452,7 +729,7 @@ int64_t kf_paged_attention_workspace_bytes(int64_t tokens, int64_t B, int64_t Hq
     using namespace kf;
     clear_error();
     if (check_shape(tokens, B, Hq, Hkv, D, max_query_len, max_context_len) != KF_OK) return -1;
-    return plan(tokens, B, Hq, Hkv, D, max_query_len, max_context_len).bytes;
+    return plan(B, Hq, Hkv, D, max_query_len, max_context_len).bytes;
 }
 
 int kf_paged_attention(const void* q, const void* key_cache, const void* value_cache, const float* key_scale,
@@ -484,7 +761,7 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
                            16 == 0 &&
                    (q_token_stride | q_head_stride) % 8 == 0,
                KF_E_INVALID, "kf_paged_attention: rows must be aligned to 16 bytes");
-    const Plan w = plan(tokens, B, Hq, Hkv, D, max_query_len, max_context_len);
+    const Plan w = plan(B, Hq, Hkv, D, max_query_len, max_context_len);
     KF_REQUIRE(w.bytes == 0 || (workspace && workspace_bytes >= w.bytes), KF_E_WORKSPACE,
                "kf_paged_attention: workspace of %lld bytes needed", (long long)w.bytes);
     PagedParams p;
@@ -498,8 +775,6 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
     p.starts = query_starts;
     p.out = out;
     p.lse = lse;
-    p.part = (float*)workspace;
-    p.ml = (float2*)((float*)workspace + tokens * Hq * w.splits * D);
     p.q_ts = q_token_stride;
     p.q_hs = q_head_stride;
     p.tokens = (int)tokens;
@@ -512,31 +787,33 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
     p.D = (int)D;
     p.shift = shift;
     p.max_q = (int)max_query_len;
-    p.row_tiles = w.row_tiles;
-    p.splits = w.splits;
     p.c = scale * kLog2e;
     p.causal = causal != 0;
     p.clear_rest = clear_rest;
+    Shares sh;
+    sh.o = (float*)workspace;
+    sh.ml = (float2*)(sh.o + w.groups * 2 * 16 * w.rt * D);
+    sh.whole = (Whole*)(sh.ml + w.groups * 2 * 16 * w.rt);
+    sh.least = w.aligned ? 1 : 4;  // a turn for each wavefront
+    sh.aligned = w.aligned;
     const hipStream_t s = (hipStream_t)stream;
     const bool e4m3 = cache_dtype == KF_CACHE_E4M3;
     if (dtype == KF_BF16)
-        e4m3 ? launch<bf16, KF_CACHE_E4M3>(p, w, s) : launch<bf16, KF_CACHE_INT8>(p, w, s);
+        e4m3 ? launch<bf16, KF_CACHE_E4M3>(p, w, sh, s) : launch<bf16, KF_CACHE_INT8>(p, w, sh, s);
     else
-        e4m3 ? launch<f16, KF_CACHE_E4M3>(p, w, s) : launch<f16, KF_CACHE_INT8>(p, w, s);
+        e4m3 ? launch<f16, KF_CACHE_E4M3>(p, w, sh, s) : launch<f16, KF_CACHE_INT8>(p, w, sh, s);
     rc = check_launch("kf_paged_attention");
-    if (rc != KF_OK || w.splits == 1) return rc;
-    const int64_t tiles16 = (max_query_len * p.G + 15) / 16;
-    const dim3 grid((unsigned)(B * tiles16), (unsigned)Hkv);
+    if (rc != KF_OK || w.aligned) return rc;
     if (dtype == KF_BF16)
-        paged_join_kernel<bf16><<<grid, 256, 0, s>>>(p, (int)tiles16);
+        launch_join<bf16>(p, w, sh, s);
     else
-        paged_join_kernel<f16><<<grid, 256, 0, s>>>(p, (int)tiles16);
+        launch_join<f16>(p, w, sh, s);
     return check_launch("kf_paged_attention (join)");
 }
 
 // Where device integers lead (paged_common.h), on the host: for the tests.
 int kfm_paged_block_of_group(const int32_t* table, int width, int blocks, int shift, int group) {
-    return kf::block_of_group(table, width, blocks, shift, group);
+    return kf::block_of_entry(kf::entry_of_group(table, width, shift, group), width, blocks, shift, group);
 }
 
 int64_t kfm_paged_block_of_slot(int64_t slot, int64_t capacity, int shift) {

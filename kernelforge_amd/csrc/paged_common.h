@@ -27,11 +27,14 @@ __host__ __device__ __forceinline__ int64_t block_of_slot(int64_t slot, int64_t 
 }
 
 // The block of a request's 16-token group, or -1 where its table (width
-// entries, at least one) names none of the cache's.
-__host__ __device__ __forceinline__ int block_of_group(const int* table, int width, int blocks, int shift, int group) {
+// entries, at least one) names none of the cache's: first what the table holds,
+// then, when that has arrived, whether it is a block.
+__host__ __device__ __forceinline__ int entry_of_group(const int* table, int width, int shift, int group) {
     const int entry = group >> (shift - 4);
-    const int id = table[entry < width ? entry : width - 1];
-    return entry < width && id >= 0 && id < blocks ? id : -1;
+    return table[entry < width ? entry : width - 1];
+}
+__host__ __device__ __forceinline__ int block_of_entry(int id, int width, int blocks, int shift, int group) {
+    return group >> (shift - 4) < width && id >= 0 && id < blocks ? id : -1;
 }
 
 // One request's place in a call of `tokens` tokens.
@@ -48,6 +51,20 @@ __host__ __device__ __forceinline__ Request request_at(const int* starts, const 
     r.n = starts ? clamp_int(starts[b + 1], r.q0, tokens) - r.q0 : 1;
     r.ctx = clamp_int(context[b], 0, kMaxContext);
     return r;
+}
+
+// The last request that starts at or before a token, or -1: the one it belongs
+// to, if it belongs to any.
+__host__ __device__ __forceinline__ int request_of(const int* starts, int B, int token) {
+    int lo = 0, hi = B;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= token)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    return lo - 1;
 }
 
 // Keys that query i of a request sees.
