@@ -1,92 +1,13 @@
-// Attention over the paged 8-bit key/value cache (layout: paged_cache.hip).
-//
-// With P the probabilities of a row and S its scores,
-//   S_j = scale ks_j <q, kcode_j>,  O = sum_j exp(S_j - max) vs_j vcode_j / sum_j exp(S_j - max),
-// ks and vs the scales of key j's block.  Codes enter the matrix products as
-// 16-bit floats without rounding; a block's key scale multiplies the fp32
-// score and its value scale the fp32 probability.
-//
-// P is rounded once, to f16 whatever q's type: p * vs / vref * 2^15 with vref
-// the largest value scale seen so far, so the product is at most 2^15 and
-// stays a normal number down to 2^-29 of the largest term (f16 rounds by at most
-// 2^-11 where bf16 would by 2^-8).  Maxima, sums and accumulators are fp32.
+// Attention over the paged cache: few rows of a request (decoding, drafts), and
+// the entry point.
 #include <type_traits>
 
-#include "paged_common.h"
+#include "paged_attn.h"
 
 namespace kf {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kPScale = 32768.0f;  // 2^15, the largest f16 operand of the second product
-constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
-
-struct PagedParams {
-    const void* q;
-    const uint8_t* kc;
-    const uint8_t* vc;
-    const float* ks;
-    const float* vs;
-    const int* tables;
-    const int* context;
-    const int* starts;  // null: one query a request
-    void* out;
-    float* lse;
-    int64_t q_ts, q_hs;
-    int tokens, B, blocks, width, Hq, Hkv, G, D, shift;
-    int max_q;
-    float c;  // scale * log2(e)
-    bool causal;
-    int clear_rest;  // rows behind the last request: 1 out, 2 lse
-};
-
-__device__ __forceinline__ Request request(const PagedParams& p, int b) {
-    return request_at(p.starts, p.context, b, p.tokens);
-}
-
-// The same for a b that is one for the wavefront: its values in scalar registers.
-__device__ __forceinline__ Request uniform_request(const PagedParams& p, int b) {
-    Request r = request(p, __builtin_amdgcn_readfirstlane(b));
-    r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
-    r.n = __builtin_amdgcn_readfirstlane(r.n);
-    r.ctx = __builtin_amdgcn_readfirstlane(r.ctx);
-    return r;
-}
-
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
-    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | lo);
-}
-
-__device__ __forceinline__ int reach(const PagedParams& p, const Request& r, int i) {
-    return keys_seen(r, i, p.causal);
-}
-
-// Keys of a request to go through: one past the table at most, since that key
-// already makes the rows that see it NaN.
-__device__ __forceinline__ int keys_to_scan(const PagedParams& p, int seen) {
-    return (int)min((int64_t)seen, ((int64_t)p.width << p.shift) + 1);
-}
-
-// Every step-th token's rows of `heads` query heads, all to one value (what: 1
-// out, 2 lse).
-template <typename T>
-__device__ __forceinline__ void fill_rows(const PagedParams& p, int from, int to, int step, int head, int heads,
-                                          int what, float value, float lse) {
-    const int vecs = p.D >> 3;
-    Vec16<T> v;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v.v[i] = (T)value;
-    for (int64_t tok = from; tok < to; tok += step) {
-        const int64_t row = tok * p.Hq + head;
-        if (what & 1)
-            for (int64_t i = threadIdx.x; i < (int64_t)heads * vecs; i += blockDim.x)
-                *(Vec16<T>*)((T*)p.out + row * p.D + 8 * i) = v;
-        if (p.lse && (what & 2))
-            for (int g = threadIdx.x; g < heads; g += blockDim.x) p.lse[(int64_t)(head + g) * p.tokens + tok] = lse;
-    }
-}
 
 // ---------------------------------------------------------------------------
 // Few rows: 16 * RT (query, head) rows of one key head are a unit of work, whose
@@ -132,8 +53,7 @@ struct Whole {
     int unused;
 };
 struct Shares {
-    float* o;     // [2 * workgroups][ROWS][D]: partial results of a workgroup's first and last segment
-    float2* ml;   // [2 * workgroups][ROWS]: running maximum (log2 units) and sum
+    Partials to;  // two of a workgroup, its first and last segment's
     Whole* whole; // [workgroups]: the unit that begins there and does not end
     int least;    // turns of a workgroup at least
     bool aligned;
@@ -143,7 +63,8 @@ struct Shares {
 template <int KEYS, int ROWS>
 __device__ __forceinline__ int2 steps_and_units(const PagedParams& p, const Request& r, bool aligned) {
     const int keys = keys_to_scan(p, r.ctx);
-    const int rows = min(r.n, p.max_q) * p.G;
+    // Requests of more rows are the prompts' kernel's.
+    const int rows = (int64_t)r.n * p.G > p.few ? 0 : min(r.n, p.max_q) * p.G;
     return make_int2(aligned ? 1 : max((keys + KEYS - 1) / KEYS, 1), (rows + ROWS - 1) / ROWS * p.Hkv);
 }
 
@@ -448,8 +369,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
                 }
 
                 // The largest value scale so far, the same on every lane.
-                float vmax = fmaxf(vscale, __shfl_xor(vscale, 16, 64));
-                vmax = fmaxf(vmax, __shfl_xor(vmax, 32, 64));
+                const float vmax = row_max4(vscale);
                 float shrink = 1.0f;
                 if (vmax > vref) {
                     shrink = vref / vmax;
@@ -472,8 +392,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
                                 s[rt][t][i] = x;
                                 most = fmaxf(most, x);
                             }
-                        most = fmaxf(most, __shfl_xor(most, 16, 64));
-                        most = fmaxf(most, __shfl_xor(most, 32, 64));
+                        most = row_max4(most);
                         const float now = fmaxf(top[rt], most);
                         const float ref = now == -__builtin_inff() ? 0.0f : now;
                         const float alpha = __builtin_amdgcn_exp2f(top[rt] - ref);
@@ -524,8 +443,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
             __syncthreads();  // the segment before has read its sums
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                sum[rt] += __shfl_xor(sum[rt], 16, 64);
-                sum[rt] += __shfl_xor(sum[rt], 32, 64);
+                sum[rt] = row_sum4(sum[rt]);
                 if (quarter == 0) {
                     sh.m[wave][16 * rt + m] = top[rt];
                     sh.l[wave][16 * rt + m] = sum[rt];
@@ -559,8 +477,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
                     }
                     if (cur.part >= 0) {
                         const int64_t at = (int64_t)cur.part * ROWS + 16 * rt + x;
-                        if (d0 == 0 && col == 0) w.ml[at] = make_float2(best, l);
-                        float* to = w.o + at * D + d0 + col;
+                        if (d0 == 0 && col == 0) w.to.ml[at] = make_float2(best, l);
+                        float* to = w.to.o + at * D + d0 + col;
                         *(f32x4*)to = (f32x4){o[0], o[1], o[2], o[3]};
                         *(f32x4*)(to + 4) = (f32x4){o[4], o[5], o[6], o[7]};
                         continue;
@@ -596,73 +514,37 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, Shares w, int unit_rows) {
     constexpr int WAYS = 128 / LANES;  // two rows a workgroup
-    __shared__ f32x4 s_o[2][256];
-    __shared__ float2 s_ml[256];
     const Whole whole = w.whole[blockIdx.x];
-    const int parts = whole.parts;
-    if (parts == 0) return;
+    if (whole.parts == 0) return;
     const int tid = threadIdx.x, col = 8 * (tid % LANES), way = tid / LANES % WAYS;
     const int x = blockIdx.y * 2 + tid / 128;  // row of the unit
     const Request r{whole.q0, whole.n, whole.ctx};
-    const int head = whole.head, row = whole.row_tile * unit_rows + x;
+    const int row = whole.row_tile * unit_rows + x;
     const bool live = row < min(r.n, p.max_q) * p.G && col < p.D;
-    float m = -__builtin_inff(), l = 0.0f;
-    f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0;
-    if (live) {
-#pragma unroll 8
-        for (int k = way; k < parts; k += WAYS) {
-            const int64_t at = (int64_t)(k == 0 ? whole.part : 2 * ((int)blockIdx.x + k)) * unit_rows + x;
-            const float2 one = w.ml[at];
-            const f32x4 y0 = *(const f32x4*)(w.o + at * p.D + col), y1 = *(const f32x4*)(w.o + at * p.D + col + 4);
-            const float now = fmaxf(m, one.x);
-            const float base = now == -__builtin_inff() ? 0.0f : now;
-            const float a = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(one.x - base);
-            l = l * a + one.y * f;
-            o0 = o0 * a + y0 * f;
-            o1 = o1 * a + y1 * f;
-            m = now;
-        }
-    }
-    s_o[0][tid] = o0;
-    s_o[1][tid] = o1;
-    s_ml[tid] = make_float2(m, l);
-    __syncthreads();
-    if (!live || way != 0) return;
-    float best = m;
-#pragma unroll
-    for (int k = 1; k < WAYS; ++k) best = fmaxf(best, s_ml[tid + k * LANES].x);
-    const float base = best == -__builtin_inff() ? 0.0f : best;
-    l = 0.0f;
-    o0 = o1 = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < WAYS; ++k) {
-        const float2 one = s_ml[tid + k * LANES];
-        const float f = __builtin_amdgcn_exp2f(one.x - base);
-        l += one.y * f;
-        o0 += s_o[0][tid + k * LANES] * f;
-        o1 += s_o[1][tid + k * LANES] * f;
-    }
-    const int i = row / p.G, token = r.q0 + i, h = head * p.G + row % p.G;
-    const bool none = reach(p, r, i) <= 0;
-    Vec16<T> v;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        v.v[k] = (T)(none ? 0.0f : o0[k] / l);
-        v.v[4 + k] = (T)(none ? 0.0f : o1[k] / l);
-    }
-    *(Vec16<T>*)((T*)p.out + ((int64_t)token * p.Hq + h) * p.D + col) = v;
-    if (p.lse && col == 0) p.lse[(int64_t)h * p.tokens + token] = none ? __builtin_inff() : (best + log2f(l)) * kLn2;
+    join_parts<T, LANES>(
+        p, w.to, live, way, col, whole.parts,
+        [&](int k) { return (int64_t)(k == 0 ? whole.part : 2 * ((int)blockIdx.x + k)) * unit_rows + x; }, r,
+        whole.head, row);
 }
 
 struct Plan {
-    int rt;
+    int rt, few;
     bool aligned;
-    int64_t groups, bytes;
+    int64_t groups, bytes;  // of the few-rows kernel
+    bool prompts;
+    PromptPlan prompt;
 };
 
-Plan plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
+// Requests of up to this many rows go to the few-rows kernel, which reads the
+// keys once for each 32 of them and spreads few units over the GPU.
+constexpr int kFewRows = 64;
+
+Plan plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
     Plan r;
-    const int64_t rows = max_q * (Hq / Hkv);
+    int64_t rows = max_q * (Hq / Hkv);
+    r.prompts = rows > kFewRows;
+    r.few = r.prompts ? kFewRows : INT32_MAX;
+    if (r.prompts) rows = kFewRows;
     r.rt = rows <= 16 || D > 128 ? 1 : 2;
     const int64_t units = B * ((rows + 16 * r.rt - 1) / (16 * r.rt)) * Hkv;
     // A second launch joins the parts of cut units (5 us).  One workgroup takes
@@ -675,6 +557,8 @@ Plan plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t 
     r.groups = device_cu_count() * (units >= device_cu_count() ? 2 : 1);
     if (r.aligned && units < r.groups) r.groups = units;
     r.bytes = r.aligned ? 0 : r.groups * (2 * 16 * r.rt * (D * 4 + 8) + sizeof(Whole));
+    r.prompt.bytes = 0;
+    if (r.prompts) r.prompt = prompt_plan(tokens, B, Hq, Hkv, D, max_ctx);
     return r;
 }
 
@@ -697,7 +581,7 @@ template <typename T, int CT> void launch(const PagedParams& p, const Plan& w, c
 
 template <typename T> void launch_join(const PagedParams& p, const Plan& w, const Shares& sh, hipStream_t s) {
     const int unit_rows = 16 * w.rt;
-    const int64_t rows = (int64_t)p.max_q * p.G < unit_rows ? (int64_t)p.max_q * p.G : unit_rows;
+    const int64_t most = (int64_t)p.max_q * p.G, rows = most < unit_rows ? most : unit_rows;
     const dim3 grid((unsigned)w.groups, (unsigned)((rows + 1) / 2));
     if (p.D <= 64)
         paged_join_kernel<T, 8><<<grid, 256, 0, s>>>(p, sh, unit_rows);
@@ -713,7 +597,8 @@ int check_shape(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
     KF_REQUIRE(Hq % Hkv == 0, KF_E_INVALID, "kf_paged_attention: Hq must be a multiple of Hkv");
     KF_REQUIRE(D >= 16 && D <= 256 && D % 16 == 0, KF_E_INVALID,
                "kf_paged_attention: head dim must be a multiple of 16 <= 256");
-    KF_REQUIRE(tokens * Hq <= INT32_MAX / 2 && B <= INT32_MAX / 2 && Hkv <= 65535 &&
+    KF_REQUIRE(tokens <= INT32_MAX / 2 && Hq <= INT32_MAX / 2 && B <= INT32_MAX / 2 && tokens * Hq <= INT32_MAX / 2 &&
+                   (tokens * (Hq / Hkv) / 64 + B) * Hkv <= INT32_MAX / 2 && Hkv <= 65535 &&
                    max_q * (Hq / Hkv) <= INT32_MAX / 2 && B * ((max_q * (Hq / Hkv) + 15) / 16) <= INT32_MAX / 2,
                KF_E_UNSUPPORTED, "kf_paged_attention: too many rows");
     return KF_OK;
@@ -729,7 +614,8 @@ int64_t kf_paged_attention_workspace_bytes(int64_t tokens, int64_t B, int64_t Hq
     using namespace kf;
     clear_error();
     if (check_shape(tokens, B, Hq, Hkv, D, max_query_len, max_context_len) != KF_OK) return -1;
-    return plan(B, Hq, Hkv, D, max_query_len, max_context_len).bytes;
+    const Plan w = plan(tokens, B, Hq, Hkv, D, max_query_len, max_context_len);
+    return w.bytes > w.prompt.bytes ? w.bytes : w.prompt.bytes;
 }
 
 int kf_paged_attention(const void* q, const void* key_cache, const void* value_cache, const float* key_scale,
@@ -761,9 +647,11 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
                            16 == 0 &&
                    (q_token_stride | q_head_stride) % 8 == 0,
                KF_E_INVALID, "kf_paged_attention: rows must be aligned to 16 bytes");
-    const Plan w = plan(B, Hq, Hkv, D, max_query_len, max_context_len);
-    KF_REQUIRE(w.bytes == 0 || (workspace && workspace_bytes >= w.bytes), KF_E_WORKSPACE,
-               "kf_paged_attention: workspace of %lld bytes needed", (long long)w.bytes);
+    const Plan w = plan(tokens, B, Hq, Hkv, D, max_query_len, max_context_len);
+    // The two kernels run one after the other and share the workspace.
+    const int64_t bytes = w.bytes > w.prompt.bytes ? w.bytes : w.prompt.bytes;
+    KF_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), KF_E_WORKSPACE,
+               "kf_paged_attention: workspace of %lld bytes needed", (long long)bytes);
     PagedParams p;
     p.q = q;
     p.kc = (const uint8_t*)key_cache;
@@ -787,13 +675,14 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
     p.D = (int)D;
     p.shift = shift;
     p.max_q = (int)max_query_len;
+    p.few = w.few;
     p.c = scale * kLog2e;
     p.causal = causal != 0;
     p.clear_rest = clear_rest;
     Shares sh;
-    sh.o = (float*)workspace;
-    sh.ml = (float2*)(sh.o + w.groups * 2 * 16 * w.rt * D);
-    sh.whole = (Whole*)(sh.ml + w.groups * 2 * 16 * w.rt);
+    sh.to.o = (float*)workspace;
+    sh.to.ml = (float2*)(sh.to.o + w.groups * 2 * 16 * w.rt * D);
+    sh.whole = (Whole*)(sh.to.ml + w.groups * 2 * 16 * w.rt);
     sh.least = w.aligned ? 1 : 4;  // a turn for each wavefront
     sh.aligned = w.aligned;
     const hipStream_t s = (hipStream_t)stream;
@@ -803,12 +692,16 @@ int kf_paged_attention(const void* q, const void* key_cache, const void* value_c
     else
         e4m3 ? launch<f16, KF_CACHE_E4M3>(p, w, sh, s) : launch<f16, KF_CACHE_INT8>(p, w, sh, s);
     rc = check_launch("kf_paged_attention");
-    if (rc != KF_OK || w.aligned) return rc;
-    if (dtype == KF_BF16)
-        launch_join<bf16>(p, w, sh, s);
-    else
-        launch_join<f16>(p, w, sh, s);
-    return check_launch("kf_paged_attention (join)");
+    if (rc != KF_OK) return rc;
+    if (!w.aligned) {
+        if (dtype == KF_BF16)
+            launch_join<bf16>(p, w, sh, s);
+        else
+            launch_join<f16>(p, w, sh, s);
+        rc = check_launch("kf_paged_attention (join)");
+        if (rc != KF_OK) return rc;
+    }
+    return w.prompts ? launch_prompt(p, w.prompt, workspace, dtype, cache_dtype, s) : KF_OK;
 }
 
 // Where device integers lead (paged_common.h), on the host: for the tests.

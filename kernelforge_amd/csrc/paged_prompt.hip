@@ -1,0 +1,432 @@
+// Attention over the paged cache: many rows of a request (chunks of prompts).
+#include <type_traits>
+
+#include "paged_attn.h"
+
+namespace kf {
+namespace {
+
+constexpr float kPromptPScale = 4096.0f;  // 2^12: a probability may exceed its row's reference by 2^kRise
+constexpr float kRise = 3.0f;
+
+// ---------------------------------------------------------------------------
+// Many rows: 64 * RT (query, head) rows of one key head per workgroup, 16 * RT a
+// wavefront, 64 keys at a time through LDS.
+//
+// The products and their operand layouts are those of the few-rows kernel
+// (paged_attn.hip): S^T = K Q^T leaves each lane the scores of one 16-token
+// group, which are the second product's operand as they are.  Here all
+// wavefronts read the same keys, so the codes go through LDS, as codes: half
+// the LDS traffic of 16-bit elements, which at 32 rows a wavefront keeps the
+// reads at half of what the LDS delivers while the matrix cores run.  Each
+// wavefront copies one of the tile's four groups (global_load_lds, 16 bytes a
+// lane), whose block, address and scales are then scalars; a tile is copied
+// while the one before it is used, with one barrier a tile.
+//
+// Keys lie in LDS as rows of DP bytes whose 16-byte chunks are permuted by
+// key_swizzle, values as the cache holds them except that odd groups have each
+// pair of 16-column tiles exchanged; both leave the 16-byte operand reads
+// without bank conflicts in 32-lane passes over 128 banks.
+// ---------------------------------------------------------------------------
+template <int DP> struct PromptShape {
+    static constexpr int RT = DP > 128 ? 1 : 2;
+    static constexpr int ROWS = 64 * RT;  // of a workgroup
+};
+
+// The permutation of a key row's 16-byte chunks.
+template <int DP> __device__ __forceinline__ int key_swizzle(int key) {
+    const int g = (key >> 4) & 3, e = key & 3;
+    if constexpr (DP == 64) return g;
+    else if constexpr (DP == 128) return 2 * g + (e >> 1);
+    else return 2 * g + 8 * (e >> 1) + (e & 1);
+}
+// The row of LDS that holds a key: with four chunks a row, odd groups exchange
+// rows 4 apart, which puts them in the other half of the banks.
+template <int DP> __device__ __forceinline__ int key_row(int key) {
+    return DP == 64 ? key ^ (((key >> 4) & 1) << 2) : key;
+}
+
+// Integers and scales that one wavefront's lanes share, through scalar loads.
+template <typename X> __device__ __forceinline__ X uniform_load(const X* p) {
+    return *(const __attribute__((address_space(4))) X*)(uintptr_t)p;
+}
+
+struct PromptWork {
+    Partials to;
+    int units, splits;
+};
+
+// A unit's key head (fastest, so that a head's units share an XCD's cache) and
+// rows.  Request b's tiles of rows begin at floor(first row / ROWS) + b, which
+// leaves room for all of them.  b: -1 where the unit has none.
+struct Unit {
+    Request r;
+    int b, head, row0;
+};
+template <int ROWS> __device__ __forceinline__ Unit unit_at(const PagedParams& p, int unit) {
+    Unit u;
+    u.head = unit % p.Hkv;
+    const int index = unit / p.Hkv;
+    auto tile_of = [&](int first, int b) { return (int)(((int64_t)first * p.G) / ROWS) + b; };
+    int b = 0;
+    for (int lo = 0, hi = p.B; lo < hi;) {
+        const int mid = (lo + hi) >> 1;
+        const int first = p.starts ? clamp_int(uniform_load(p.starts + mid), 0, p.tokens) : mid;
+        if (tile_of(first, mid) <= index) {
+            b = mid;
+            lo = mid + 1;
+        } else {
+            hi = mid;
+        }
+    }
+    u.b = __builtin_amdgcn_readfirstlane(b);
+    u.r = uniform_request(p, u.b);
+    const int row_tile = index - tile_of(u.r.q0, u.b);
+    u.row0 = row_tile * ROWS;
+    if ((int64_t)u.r.n * p.G <= p.few || row_tile < 0 || u.row0 >= min(u.r.n, p.max_q) * p.G) u.b = -1;
+    return u;
+}
+
+template <typename T, int CT, int DP>
+__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, PromptWork w) {
+    constexpr int RT = PromptShape<DP>::RT, ROWS = PromptShape<DP>::ROWS;
+    constexpr int KC = DP / 64, VT = DP / 16, CH = DP / 16;
+    constexpr int TILE = 64 * DP;  // bytes of a tile's keys or values
+    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][TILE];
+    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][TILE];
+    __shared__ float2 s_scales[2][4];  // key scale (NaN: no such block), value scale
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, quarter = lane >> 4;
+    const int D = p.D;
+
+    // The latest units, which see the most keys, go first.
+    const Unit u = unit_at<ROWS>(p, w.units - 1 - blockIdx.x);
+    const Request r = u.r;
+    const int b = u.b, head = u.head, row0 = u.row0, rows = min(r.n, p.max_q) * p.G;
+    if (u.b < 0) return;
+    if (row0 == 0 && blockIdx.y == 0 && r.n > p.max_q)
+        fill_rows<T>(p, r.q0 + p.max_q, r.q0 + r.n, 1, head * p.G, p.G, 3, __builtin_nanf(""), __builtin_nanf(""));
+
+    // This wavefront's rows.
+    const int my_row0 = row0 + 16 * RT * wave;
+    int limit[RT];
+    typename V<T>::x8 qf[RT][KC][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = my_row0 + 16 * rt + m, i = row / p.G;
+        const bool live = row < rows;
+        limit[rt] = live ? reach(p, r, i) : 0;
+        const T* q = (const T*)p.q + (int64_t)(r.q0 + i) * p.q_ts + (int64_t)(head * p.G + row % p.G) * p.q_hs;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int col = 64 * c + 16 * quarter + 8 * h;
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (live && col < D) v = *(const u32x4*)(q + col);
+                qf[rt][c][h] = __builtin_bit_cast(typename V<T>::x8, v);
+            }
+    }
+    auto seen_by = [&](int row) {
+        return __builtin_amdgcn_readfirstlane(keys_to_scan(p, reach(p, r, min(row, rows - 1) / p.G)));
+    };
+    // Keys that the wavefront's rows all see, and that any sees.
+    const int all_see = my_row0 < rows ? __builtin_amdgcn_readfirstlane(reach(p, r, my_row0 / p.G)) : 0;
+    const int any_sees = my_row0 < rows ? seen_by(my_row0 + 16 * RT - 1) : 0;
+    const int tiles = (seen_by(row0 + ROWS - 1) + 63) >> 6;
+    const int first = (int)((int64_t)tiles * blockIdx.y / w.splits);
+    const int last = (int)((int64_t)tiles * (blockIdx.y + 1) / w.splits);
+
+    // Copies of this wavefront's group.  Lane i of instruction j fills the group's
+    // 16-byte slot 64 j + i.
+    const int subs = (1 << (p.shift - 4)) - 1;
+    const int64_t unit_bytes = (int64_t)D << p.shift;
+    uint32_t from_k[DP / 64], from_v[DP / 64];
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+        const int slot = 64 * j + lane;
+        const int key = key_row<DP>(16 * wave + slot / CH);  // an exchange is its own inverse
+        const int chunk = (slot % CH) ^ key_swizzle<DP>(key);
+        from_k[j] = (key & 15) * D + (16 * chunk < D ? 16 * chunk : 0);  // past D: any bytes, the query is 0 there
+        const int col = slot ^ ((wave & 1) << 4);
+        from_v[j] = 16 * (col < D ? col : 0);  // past D: columns that are not written
+    }
+    const int* table = p.tables + (int64_t)b * p.width;
+    auto entry_of = [&](int tile) {
+        const int entry = (4 * tile + wave) >> (p.shift - 4);
+        return uniform_load(table + min(entry, p.width - 1));
+    };
+    auto block_of = [&](int id, int tile) {
+        return __builtin_amdgcn_readfirstlane(block_of_entry(id, p.width, p.blocks, p.shift, 4 * tile + wave));
+    };
+    const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_addr(&s_keys[0][0])) + wave * 16 * DP;
+    const uint32_t lds_v = __builtin_amdgcn_readfirstlane(lds_addr(&s_values[0][0])) + wave * 16 * DP;
+    auto copy_tile = [&](int tile, int block) {
+        const int64_t at = ((int64_t)max(block, 0) * p.Hkv + head) * unit_bytes + 16 * ((4 * tile + wave) & subs) * D;
+        const uint32_t buffer = (tile & 1) * TILE;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            lds_copy16_sbase(p.kc + at, from_k[j], lds_k + buffer + 1024 * j);
+            lds_copy16_sbase(p.vc + at, from_v[j], lds_v + buffer + 1024 * j);
+        }
+    };
+    auto scales_of = [&](int tile, int block) {
+        const int64_t at = (int64_t)max(block, 0) * p.Hkv + head;
+        const float vs = uniform_load(p.vs + at);
+        float2 s = make_float2(uniform_load(p.ks + at) * p.c, vs < __builtin_inff() ? vs : __builtin_nanf(""));
+        if (block < 0) s = make_float2(__builtin_nanf(""), 0.0f);
+        if (64 * tile + 16 * wave >= r.ctx) s = make_float2(0.0f, 0.0f);  // says nothing
+        return s;
+    };
+
+    f32x4 acc[RT][VT];
+    float ref[RT], sum[RT], vref = kLeastScale, inv_vref = 1.0f / kLeastScale;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        ref[rt] = -__builtin_inff();
+        sum[rt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < VT; ++d) acc[rt][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // Operand reads: a lane's chunk of column block c, and its values of the even
+    // and of the odd column tiles.
+    uint32_t read_k[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+        const int key = 16 * (m >> 2) + (m & 3);
+        read_k[c] = key * DP + 16 * ((4 * c + quarter) ^ key_swizzle<DP>(key));
+    }
+    const int exchange = DP == 64 ? ((m >> 2) & 1) << 2 : 0;  // of the rows 4t of odd groups
+    const uint32_t read_v = quarter * 16 * DP + 16 * m;
+    const int swap = (quarter & 1) << 8;
+
+    int block = -1, ahead = 0;
+    if (first < last) {
+        block = block_of(entry_of(first), first);
+        copy_tile(first, block);
+        ahead = entry_of(min(first + 1, last - 1));
+        const float2 s = scales_of(first, block);
+        if (lane == 0) s_scales[first & 1][wave] = s;
+    }
+    for (int tile = first; tile < last; ++tile) {
+        const int now = tile & 1;
+        wait_vmem();  // this wavefront's group has arrived
+        {
+            // Values behind the context or of no block are zeroed: what lies there may be NaN.
+            const int valid = block < 0 ? 0 : clamp_int(r.ctx - (64 * tile + 16 * wave), 0, 16);
+            if (valid < 16) {
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {
+                    u32x4* at = (u32x4*)&s_values[now][wave * 16 * DP + 16 * (64 * j + lane)];
+                    u32x4 v = *at;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int bytes = clamp_int(valid - 4 * e, 0, 4);
+                        v[e] &= bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1u;
+                    }
+                    *at = v;
+                }
+            }
+        }
+        __syncthreads();
+        float2 next_scales = make_float2(0.0f, 0.0f);
+        if (tile + 1 < last) {
+            block = block_of(ahead, tile + 1);
+            copy_tile(tile + 1, block);
+            ahead = entry_of(min(tile + 2, last - 1));
+            next_scales = scales_of(tile + 1, block);
+        }
+        if (64 * tile < any_sees) {
+            const uint8_t* keys = s_keys[now];
+            const uint8_t* values = s_values[now];
+            const float2 mine = s_scales[now][quarter];
+            float vmax = fmaxf(fmaxf(s_scales[now][0].y, s_scales[now][1].y),
+                               fmaxf(s_scales[now][2].y, s_scales[now][3].y));
+            f32x4 s[RT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const u32x4 k = *(const u32x4*)(keys + read_k[c] + ((4 * t) ^ exchange) * DP);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const auto a = Codes<T, CT>::x8(k[2 * h], k[2 * h + 1]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c][h], s[rt][t]);
+                    }
+                }
+            }
+            const int key0 = 64 * tile + 16 * quarter;  // position of this lane's first key
+            const bool edge = 64 * tile + 64 > all_see;
+            float most[RT];
+            bool rise = false;
+            auto scale_scores = [&](auto at_edge) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    most[rt] = -__builtin_inff();
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float x = s[rt][t][i] * mine.x;
+                            if (decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt]) x = -__builtin_inff();
+                            s[rt][t][i] = x;
+                            most[rt] = fmaxf(most[rt], x);
+                        }
+                    most[rt] = row_max4(most[rt]);
+                    rise |= most[rt] > ref[rt] + kRise;
+                }
+            };
+            if (edge)
+                scale_scores(std::true_type());
+            else
+                scale_scores(std::false_type());
+            // The references follow the rows' maxima when one has risen by 2^kRise.
+            if (__any(rise) || vmax > vref) {
+                const float shrink = vmax > vref ? vref / vmax : 1.0f;
+                if (vmax > vref) {
+                    vref = vmax;
+                    inv_vref = 1.0f / vmax;
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float to = fmaxf(ref[rt], most[rt]);
+                    const float alpha = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
+                    ref[rt] = to;
+                    sum[rt] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < VT; ++d) acc[rt][d] *= alpha * shrink;
+                }
+            }
+            const float factor = mine.y * inv_vref * kPromptPScale;
+            V<f16>::x8 pf[RT][2];
+            auto probabilities = [&](auto at_edge) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float base = ref[rt] == -__builtin_inff() ? 0.0f : ref[rt];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - base);
+                            sum[rt] += e;
+                            // A hidden key's weight is 0 whatever its block's scale.
+                            const float x =
+                                decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt] ? 0.0f : e * factor;
+                            pf[rt][t >> 1][4 * (t & 1) + i] = (f16)x;
+                        }
+                }
+            };
+            if (edge)
+                probabilities(std::true_type());
+            else
+                probabilities(std::false_type());
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+                const u32x4 v = *(const u32x4*)(values + read_v + 256 * d + (d & 1 ? -swap : swap));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const auto a = Codes<f16, CT>::x8(v[2 * h], v[2 * h + 1]);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
+                }
+            }
+        }
+        if (tile + 1 < last && lane == 0) s_scales[now ^ 1][wave] = next_scales;
+    }
+
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = my_row0 + 16 * rt + m;
+        const float l = row_sum4(sum[rt]);
+        if (row >= rows) continue;
+        const int i = row / p.G, token = r.q0 + i, h = head * p.G + row % p.G;
+        if (w.splits > 1) {
+            const int64_t at = ((int64_t)blockIdx.x * w.splits + blockIdx.y) * ROWS + (row - row0);
+            if (quarter == 0) w.to.ml[at] = make_float2(ref[rt], l);
+#pragma unroll
+            for (int d = 0; d < VT; ++d)
+                if (16 * d < D)
+                    *(f32x4*)(w.to.o + at * D + 16 * d + 4 * quarter) = acc[rt][d] * (1.0f / kPromptPScale) * vref;
+            continue;
+        }
+        const bool none = limit[rt] <= 0;
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+            if (16 * d >= D) continue;
+            const f32x4 o = acc[rt][d] * (1.0f / kPromptPScale) * vref;
+            typename V<T>::x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] / l);
+            *(typename V<T>::x4*)((T*)p.out + ((int64_t)token * p.Hq + h) * D + 16 * d + 4 * quarter) = v;
+        }
+        if (p.lse && quarter == 0)
+            p.lse[(int64_t)h * p.tokens + token] = none ? __builtin_inff() : (ref[rt] + log2f(l)) * kLn2;
+    }
+}
+
+// Joins a unit's splits, in order: two rows a workgroup, LANES threads with eight
+// columns each a row, WAYS sets of them that take every WAYS-th split.
+template <typename T, int ROWS, int LANES>
+__global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedParams p, PromptWork w) {
+    constexpr int WAYS = 128 / LANES;
+    const Unit u = unit_at<ROWS>(p, w.units - 1 - blockIdx.x);
+    if (u.b < 0) return;
+    const int tid = threadIdx.x, col = 8 * (tid % LANES), way = tid / LANES % WAYS;
+    const int x = blockIdx.y * 2 + tid / 128, row = u.row0 + x;
+    const bool live = row < min(u.r.n, p.max_q) * p.G && col < p.D;
+    join_parts<T, LANES>(
+        p, w.to, live, way, col, w.splits,
+        [&](int k) { return ((int64_t)blockIdx.x * w.splits + k) * ROWS + x; }, u.r, u.head, row);
+}
+
+template <typename T, int CT, int DP>
+int launch_shape(const PagedParams& p, const PromptWork& w, hipStream_t s) {
+    constexpr int ROWS = PromptShape<DP>::ROWS;
+    paged_prompt_kernel<T, CT, DP><<<dim3((unsigned)w.units, (unsigned)w.splits), 256, 0, s>>>(p, w);
+    int rc = check_launch("kf_paged_attention (prompts)");
+    if (rc != KF_OK || w.splits == 1) return rc;
+    paged_prompt_join_kernel<T, ROWS, DP / 8><<<dim3((unsigned)w.units, ROWS / 2), 256, 0, s>>>(p, w);
+    return check_launch("kf_paged_attention (prompts' join)");
+}
+
+template <typename T, int CT> int launch_dim(const PagedParams& p, const PromptWork& w, hipStream_t s) {
+    if (p.D <= 64) return launch_shape<T, CT, 64>(p, w, s);
+    if (p.D <= 128) return launch_shape<T, CT, 128>(p, w, s);
+    return launch_shape<T, CT, 256>(p, w, s);
+}
+
+int unit_rows(int64_t D) { return D > 128 ? PromptShape<256>::ROWS : PromptShape<128>::ROWS; }
+
+}  // namespace
+
+PromptPlan prompt_plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_ctx) {
+    PromptPlan w;
+    const int rows = unit_rows(D);
+    w.units = (tokens * (Hq / Hkv) / rows + B) * Hkv;
+    // Two workgroups a CU fit; fewer units than CUs have their keys split.
+    int64_t splits = w.units >= device_cu_count() ? 1 : (2 * device_cu_count() + w.units - 1) / w.units;
+    const int64_t most = max_ctx / 512;
+    if (splits > most) splits = most;
+    w.splits = splits > 1 ? (int)splits : 1;
+    w.bytes = w.splits > 1 ? w.units * w.splits * rows * (D * 4 + 8) : 0;
+    return w;
+}
+
+int launch_prompt(const PagedParams& p, const PromptPlan& plan, void* workspace, int dtype, int cache_dtype,
+                  hipStream_t stream) {
+    PromptWork w;
+    w.to.o = (float*)workspace;
+    w.to.ml = (float2*)(w.to.o + plan.units * plan.splits * unit_rows(p.D) * p.D);
+    w.units = (int)plan.units;
+    w.splits = plan.splits;
+    const bool e4m3 = cache_dtype == KF_CACHE_E4M3;
+    if (dtype == KF_BF16)
+        return e4m3 ? launch_dim<bf16, KF_CACHE_E4M3>(p, w, stream) : launch_dim<bf16, KF_CACHE_INT8>(p, w, stream);
+    return e4m3 ? launch_dim<f16, KF_CACHE_E4M3>(p, w, stream) : launch_dim<f16, KF_CACHE_INT8>(p, w, stream);
+}
+
+}  // namespace kf

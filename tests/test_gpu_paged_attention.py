@@ -10,10 +10,13 @@ Z = max_j sum_d |q_d||k_jd| * scale:
     minus the maximum in log2 units (2^-24 times its size, at most 2 Z log2 e):
     e = (D + 8) 2^-24 * Z bounds the error of a score, and 2 e that of log p;
   - exp2 adds 2^-22, the join of the parts as much again;
-  - a probability is rounded to f16: 2^-11 of it, 2^-40 of the largest value
-    below f16's normal numbers;
+  - a probability, times 2^12 (chunks of prompts; few rows: 2^15) and its block's
+    value scale over the largest one, is rounded to f16: 2^-11 of it, or below
+    f16's normal numbers (2^-14) half a step of 2^-24, which is 2^-37 of a key of
+    the largest value; n keys: n 2^-37 of it, after the division by a sum of at
+    least 1;
   - the sums add n 2^-24 of A.
-So |out - exact| <= h |exact| + A (2 e + 2^-21 + 2^-11 + 2 n 2^-24) + 2^-39 max|v|,
+So |out - exact| <= h |exact| + A (2 e + 2^-21 + 2^-11 + 2 n 2^-24) + n 2^-37 max|v|,
 |lse - exact| <= 2 e + 2^-21 + n 2^-24 + 4 * 2^-24 |lse|.
 """
 
@@ -56,7 +59,7 @@ def bounds(want, out_dtype, cache, D, n):
     e = (D + 8) * 2.0 ** -24 * slack
     top = float((orc.LARGEST[cache[0].dtype] + 1) * cache[3].abs().nan_to_num(0).max())
     rel = 2 * e.T[..., None] + 2.0 ** -21 + 2.0 ** -11 + 2 * n * 2.0 ** -24
-    return half * out.abs().clamp(min=least) + spread * rel + 2.0 ** -39 * top, 2 * e + 2.0 ** -21 + n * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
+    return half * out.abs().clamp(min=least) + spread * rel + n * 2.0 ** -37 * top, 2 * e + 2.0 ** -21 + n * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
 
 
 def compare(got, want, limits):
@@ -136,6 +139,39 @@ def test_ragged(T, Hq, Hkv, D, dtype, code, causal):
     if causal:  # the first three of five tokens over two keys see none
         assert not out[1:4].any() and lse[:, 1:4].isposinf().all()
     assert not out[-2:].any() and lse[:, -2:].isposinf().all()
+
+
+@pytest.mark.parametrize("code,dtype", [(E4M3, torch.bfloat16), (INT8, torch.float16)])
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(16, 8, 2, 128), (64, 4, 4, 64), (32, 8, 1, 256), (128, 6, 2, 80), (16, 3, 1, 16),
+                                        (32, 7, 7, 208)])
+def test_prompts(T, Hq, Hkv, D, code, dtype):
+    """Chunks of prompts over contexts long enough to be split, beside a decoding
+    request and one at the border of the kernels (64 and 65 rows of a key head):
+    several tiles of rows, tiles that end inside a block, rows of two queries."""
+    rng = random.Random(D)
+    group = Hq // Hkv
+    count = [1, 64 // group, 64 // group + 1, 150, 33]
+    context = [1200, 700, 1030, 1800, 33]
+    starts = [0]
+    for n in count:
+        starts.append(starts[-1] + n)
+    cache = make_cache(400, Hkv, T, D, code)
+    tables = layout(context, T, 400, rng)
+    q = queries(starts[-1], Hq, D, dtype)
+    check(q, cache, tables, context, starts, max_query_len=150)
+    check(q, cache, tables, context, starts, causal=False, max_context_len=100)
+
+
+def test_prompt_scores_that_grow():
+    """Scores that rise past the rows' references again and again, and value scales
+    that do."""
+    T, D, c, n = 16, 64, 800, 60
+    cache = make_cache(50, 1, T, D, INT8, spread=0.0)
+    order = list(range(50))
+    cache.key_scale[:, 0] = torch.linspace(0.001, 0.2, 50).to(DEV)
+    cache.value_scale[:, 0] = 2.0 ** torch.linspace(-30, 3, 50).to(DEV)
+    check(queries(n, 4, D, torch.bfloat16), cache, [order], [c], [0, n])
+    check(queries(n, 4, D, torch.float16), cache, [order[::-1]], [c], [0, n], scale=0.5)
 
 
 @pytest.mark.parametrize("max_context_len", [0, 64, 700, 5000, None])
