@@ -202,9 +202,11 @@ template <> struct Code<KF_CACHE_INT8> {
     static constexpr int kExponent = 6;
     static __device__ __forceinline__ uint32_t pack(const float* x) {
         uint32_t r = 0;
+        // Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and
+        // leaves it in the low byte.
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            r |= ((uint32_t)(int)rintf(fminf(fmaxf(x[i], -kMost), kMost)) & 0xffu) << (8 * i);
+            r |= (__float_as_uint(fminf(fmaxf(x[i], -kMost), kMost) + 12582912.0f) & 0xffu) << (8 * i);
         return r;
     }
     static __device__ __forceinline__ void unpack(uint32_t c, float* x) {
@@ -265,6 +267,18 @@ template <typename T> struct alignas(4) Pair {
     T v[2];
 };
 
+// Which of the call's tokens fills a slot of the run's block: for consecutive
+// slots, as a request's tokens have, arithmetic; else a table in LDS.
+struct Run {
+    int first, count;   // its slots, where they are consecutive
+    const int* winner;  // else the last token of the run that names a slot, or -1
+    __device__ __forceinline__ int token(int slot) const {
+        if (winner) return winner[slot];
+        const int k = slot - first;
+        return k >= 0 && k < count ? k : -1;
+    }
+};
+
 // T: element type of the new keys and values; CT: the cache's; DC: the head
 // dim's class (64, 128 or 256).  blockDim.x = 64 * max(4, block_tokens / 16).
 template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void paged_append_kernel(AppendParams p) {
@@ -272,9 +286,8 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
     constexpr int NT = DC == 64 ? 8 : 16;   // tokens of a value group per lane
     constexpr int PI = DC == 256 ? 2 : 1;   // column pairs per lane
     __shared__ int s_winner[128];
-    __shared__ int s_end;
     __shared__ uint32_t s_max[8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bt = 1 << p.shift, groups = bt >> 4, D = p.D;
     const int unit = blockIdx.y * ((int)(blockDim.x >> 6) / groups) + wave / groups;
     const int g = wave % groups;
@@ -282,30 +295,46 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
     const int part = active && unit >= p.Hkv ? 1 : 0;
     const int head = active ? unit - part * p.Hkv : 0;
 
+    // The tokens of this workgroup's slice at which a run begins.
     const int64_t t_begin = (int64_t)blockIdx.x * p.slice;
-    const int64_t t_stop = min(t_begin + p.slice, p.tokens);
-    for (int64_t t = t_begin; t < t_stop; ++t) {
-        const int64_t block = block_of_slot(p.slots[t], p.capacity, p.shift);
-        if (block < 0 || (t > 0 && block_of_slot(p.slots[t - 1], p.capacity, p.shift) == block)) continue;
+    const int in_slice = (int)min((int64_t)p.slice, p.tokens - t_begin);
+    auto block_at = [&](int64_t t) {
+        return t >= 0 && t < p.tokens ? block_of_slot(p.slots[t], p.capacity, p.shift) : (int64_t)-1;
+    };
+    const int64_t mine = lane < in_slice ? block_at(t_begin + lane) : -1;
+    int64_t before = __shfl_up((long long)mine, 1, 64);
+    if (lane == 0) before = block_at(t_begin - 1);
+    uint64_t begins = __ballot(mine >= 0 && mine != before);
 
-        // The run's end, then for each slot of the block the last token that names it.
-        __syncthreads();
-        for (int i = tid; i < bt; i += blockDim.x) s_winner[i] = -1;
-        if (tid == 0) s_end = INT_MAX;
+    while (begins) {
+        const int64_t t = t_begin + __builtin_ctzll(begins);
+        begins &= begins - 1;
+        // The run's length, and whether its slots are consecutive.
+        const int64_t slot = p.slots[t], block = slot >> p.shift;
         int length = 0;
-        for (int64_t base = t;; base += blockDim.x) {
-            __syncthreads();
-            const int64_t i = base + tid;
-            const bool in = i < p.tokens && block_of_slot(p.slots[i], p.capacity, p.shift) == block;
-            const uint64_t out = __ballot(!in);
-            if (out && lane == 0) atomicMin(&s_end, (int)(base - t) + wave * 64 + __builtin_ctzll(out));
-            __syncthreads();
-            length = s_end;
-            if (length != INT_MAX) break;  // found at the call's last token at the latest
+        bool consecutive = true;
+        for (;; length += 64) {
+            const int64_t i = t + length + lane;
+            const int64_t s = i < p.tokens ? p.slots[i] : -1;
+            const bool in = block_of_slot(s, p.capacity, p.shift) == block;
+            const uint64_t out = __ballot(!in), other = __ballot(in && s != slot + length + lane);
+            const int here = out ? __builtin_ctzll(out) : 64;
+            consecutive &= (here == 64 ? other : other & ((1ull << here) - 1)) == 0;
+            if (out) {
+                length += here;
+                break;  // at the call's last token at the latest
+            }
         }
-        for (int i = tid; i < length; i += blockDim.x) atomicMax(&s_winner[p.slots[t + i] & (bt - 1)], i);
-        __syncthreads();
-        const bool begun = s_winner[0] >= 0;
+        Run run{(int)(slot & (bt - 1)), length, nullptr};
+        if (!consecutive) {  // the same for all of the workgroup's wavefronts
+            __syncthreads();
+            for (int i = tid; i < bt; i += blockDim.x) s_winner[i] = -1;
+            __syncthreads();
+            for (int i = tid; i < length; i += blockDim.x) atomicMax(&s_winner[p.slots[t + i] & (bt - 1)], i);
+            __syncthreads();
+            run.winner = s_winner;
+        }
+        const bool begun = run.token(0) >= 0;
 
         const int64_t where = block * p.Hkv + head;
         const float old_scale = active ? p.scales[part][where] : 0.0f;
@@ -313,50 +342,38 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
         const int64_t ts = p.token_stride[part];
         uint8_t* codes = p.codes[part] + where * bt * D + g * 16 * D;
         uint32_t most = 0;
+        float stored;
 
-        // Keys: vector c of the group is 8 columns of token c / (D/8).
-        Vec16<T> kx[KI];
-        int win[KI];
-        // Values: lane (pair, part of the group) holds two columns of NT tokens.
-        Pair<T> vx[PI][NT];
-        const int pairs = DC == 64 ? 32 : 64;
-        const int vcol = 2 * (lane % pairs), vtok = DC == 64 ? 8 * (lane / pairs) : 0;
-        if (active && part == 0) {
+        // All of a unit's wavefronts meet here.
+        auto scale_of = [&]() {
+            most = wave_max_u32(most);
+            if (groups > 1) {
+                __syncthreads();  // the run before has read its maxima
+                if (lane == 0) s_max[wave] = most;
+                __syncthreads();
+                for (int w = 0; w < groups; ++w) most = max(most, s_max[wave - g + w]);
+            }
+            return unit_scale<CT>(most, old_scale, begun, &stored);
+        };
+
+        if (part == 0) {
+            // Keys: vector c of the group is 8 columns of token c / (D/8).
+            Vec16<T> kx[KI];
+            int win[KI];
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
-                const int c = lane + 64 * i, tok = c / (D >> 3), col = 8 * (c % (D >> 3));
-                win[i] = tok < 16 ? s_winner[g * 16 + tok] : -1;
+                const int c = lane + 64 * i, tok = c / (D >> 3), col = 8 * (c - tok * (D >> 3));
+                win[i] = active && tok < 16 ? run.token(g * 16 + tok) : -1;
+                if (win[i] >= 0) kx[i] = *(const Vec16<T>*)(x + win[i] * ts + col);
+            }
+#pragma unroll
+            for (int i = 0; i < KI; ++i)
                 if (win[i] >= 0) {
-                    kx[i] = *(const Vec16<T>*)(x + win[i] * ts + col);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) most = max(most, magnitude_bits(kx[i].v[k]));
                 }
-            }
-        } else if (active) {
-#pragma unroll
-            for (int q = 0; q < PI; ++q) {
-                const int col = vcol + 128 * q;
-#pragma unroll
-                for (int k = 0; k < NT; ++k) {
-                    const int w = s_winner[g * 16 + vtok + k];
-                    vx[q][k].v[0] = vx[q][k].v[1] = (T)0.0f;
-                    if (w >= 0 && col < D) vx[q][k] = *(const Pair<T>*)(x + w * ts + col);
-                    most = max(most, max(magnitude_bits(vx[q][k].v[0]), magnitude_bits(vx[q][k].v[1])));
-                }
-            }
-        }
-        most = wave_max_u32(most);
-        if (groups > 1) {
-            if (lane == 0) s_max[wave] = most;
-            __syncthreads();
-            for (int w = 0; w < groups; ++w) most = max(most, s_max[wave - g + w]);
-        }
-        if (!active) continue;
-        float stored;
-        const UnitScale u = unit_scale<CT>(most, old_scale, begun, &stored);
-        if (g == 0 && lane == 0) p.scales[part][where] = stored;
-
-        if (part == 0) {
+            const UnitScale u = scale_of();
+            if (!active) continue;
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
                 const int c = lane + 64 * i;
@@ -378,33 +395,63 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
                 *to = r;
             }
         } else {
+            // Values: lane (pair, part of the group) holds two columns of NT tokens.
+            const int pairs = DC == 64 ? 32 : 64;
+            const int vcol = 2 * (lane % pairs), vtok = DC == 64 ? 8 * (lane / pairs) : 0;
+            Pair<T> vx[PI][NT];
+            uint32_t have = 0;  // tokens of the call, a bit each
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const int w = run.token(g * 16 + vtok + k);
+                if (w >= 0) have |= 1u << k;
+#pragma unroll
+                for (int q = 0; q < PI; ++q) {
+                    const int col = vcol + 128 * q;
+                    vx[q][k].v[0] = vx[q][k].v[1] = (T)0.0f;
+                    if (w >= 0 && col < D) vx[q][k] = *(const Pair<T>*)(x + w * ts + col);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < PI; ++q)
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+                    most = max(most, max(magnitude_bits(vx[q][k].v[0]), magnitude_bits(vx[q][k].v[1])));
+            const UnitScale u = scale_of();
+            const bool all = have == (1u << NT) - 1u;
 #pragma unroll
             for (int q = 0; q < PI; ++q) {
                 const int col = vcol + 128 * q;
                 if (col >= D) continue;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    uint32_t* to = (uint32_t*)(codes + (col + e) * 16 + vtok);
+                    typedef uint32_t words __attribute__((ext_vector_type(NT / 4)));
+                    words* to = (words*)(codes + (col + e) * 16 + vtok);
+                    words r;
 #pragma unroll
                     for (int k4 = 0; k4 < NT / 4; ++k4) {
                         float y[4];
-                        uint32_t keep = 0;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            y[k] = u.finite ? (float)vx[q][4 * k4 + k].v[e] * u.inverse : 0.0f;
-                            if (s_winner[g * 16 + vtok + 4 * k4 + k] < 0) keep |= 0xffu << (8 * k);
-                        }
-                        uint32_t r = Code<CT>::pack(y) & ~keep;
-                        if (keep && !begun) {
-                            if (keep == 0xffffffffu && u.ratio == 1.0f) continue;
-                            const uint32_t held = to[k4];
-                            r |= (u.ratio == 1.0f ? held : rescale<CT>(held, u.ratio)) & keep;
-                        }
-                        to[k4] = r;
+                        for (int k = 0; k < 4; ++k) y[k] = u.finite ? (float)vx[q][4 * k4 + k].v[e] * u.inverse : 0.0f;
+                        r[k4] = Code<CT>::pack(y);
                     }
+                    if (!all) {
+                        if (have == 0 && !begun && u.ratio == 1.0f) continue;
+                        words held = {};
+                        if (!begun) held = *to;
+#pragma unroll
+                        for (int k4 = 0; k4 < NT / 4; ++k4) {
+                            uint32_t mine = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mine |= have >> (4 * k4 + k) & 1 ? 0xffu << (8 * k) : 0u;
+                            const uint32_t keep = u.ratio == 1.0f || begun ? held[k4] : rescale<CT>(held[k4], u.ratio);
+                            r[k4] = (r[k4] & mine) | (keep & ~mine);
+                        }
+                    }
+                    *to = r;
                 }
             }
         }
+        if (g == 0 && lane == 0) p.scales[part][where] = stored;
     }
 }
 
@@ -495,8 +542,9 @@ int kf_paged_cache_append(const void* key, const void* value, const int64_t* slo
     const int groups = 1 << (shift - 4), waves = groups > 4 ? groups : 4;
     const int64_t gy = (2 * Hkv * groups + waves - 1) / waves;
     // Decoding gives every token a block of its own: a workgroup each.  Prompts
-    // start a run every block_tokens tokens: a workgroup for as many.
-    p.slice = tokens * gy > 4096 ? 1 << shift : 1;
+    // start a run every block_tokens tokens: a workgroup for as many (64 at most,
+    // the lanes that look for a run's start).
+    p.slice = tokens * gy <= 4096 ? 1 : shift < 6 ? 1 << shift : 64;
     const int64_t gx = (tokens + p.slice - 1) / p.slice;
     const dim3 grid((unsigned)gx, (unsigned)gy);
     const hipStream_t s = (hipStream_t)stream;
