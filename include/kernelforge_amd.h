@@ -543,10 +543,11 @@ int kf_paged_block_tables(int32_t* block_tables, const int32_t* context_lens, co
  * block gives NaN, until the block is started again.
  *
  * key, value: [tokens, Hkv, D] of `dtype` (f16 or bf16) with the given strides
- * in elements (multiples of 8; the dim is contiguous, 16-byte aligned).
- * Slots outside the cache are skipped.  The tokens of one block must follow
- * one another in the call, as the tokens of one request do (of two that name
- * one slot the later is kept); else the codes of that block are unspecified.
+ * in elements (multiples of 8, those of tokens below 2^26; the dim is
+ * contiguous, 16-byte aligned).  Slots outside the cache are skipped.
+ * The tokens of one block must follow one another in the call, as the tokens
+ * of one request do (of two that name one slot the later is kept); else the
+ * codes of that block are unspecified.
  */
 int kf_paged_cache_append(const void* key, const void* value, const int64_t* slots, void* key_cache,
                           void* value_cache, float* key_scale, float* value_scale, int64_t tokens, int64_t blocks,

@@ -170,7 +170,8 @@ struct AppendParams {
     const void* x[2];  // key, value
     uint8_t* codes[2];
     float* scales[2];
-    int64_t token_stride[2], head_stride[2];
+    int token_stride[2];
+    int64_t head_stride[2];
     const int64_t* slots;
     int64_t tokens, capacity;  // capacity: slots of the cache
     int Hkv, D, shift, slice;
@@ -181,13 +182,10 @@ template <> struct Code<KF_CACHE_E4M3> {
     static constexpr float kMost = 448.0f;
     static constexpr uint32_t kMantissa = 0x600000u;  // 448 = 1.75 * 2^8
     static constexpr int kExponent = 8;
-    // Four scaled values as codes, in order from the low byte.
+    // Four values of at most kMost as codes, in order from the low byte.
     static __device__ __forceinline__ uint32_t pack(const float* x) {
-        float c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = fminf(fmaxf(x[i], -kMost), kMost);
-        int r = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], r, true);
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
     }
     static __device__ __forceinline__ void unpack(uint32_t c, float* x) {
         x[0] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
@@ -206,7 +204,7 @@ template <> struct Code<KF_CACHE_INT8> {
         // leaves it in the low byte.
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            r |= (__float_as_uint(fminf(fmaxf(x[i], -kMost), kMost) + 12582912.0f) & 0xffu) << (8 * i);
+            r |= (__float_as_uint(x[i] + 12582912.0f) & 0xffu) << (8 * i);
         return r;
     }
     static __device__ __forceinline__ void unpack(uint32_t c, float* x) {
@@ -226,7 +224,7 @@ template <int CT> __device__ __forceinline__ uint32_t rescale(uint32_t c, float 
     float x[4];
     Code<CT>::unpack(c, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] *= ratio;
+    for (int i = 0; i < 4; ++i) x[i] = fminf(fmaxf(x[i] * ratio, -Code<CT>::kMost), Code<CT>::kMost);
     return Code<CT>::pack(x);
 }
 
@@ -252,9 +250,17 @@ __device__ __forceinline__ UnitScale unit_scale(uint32_t magnitude, float old_sc
     return u;
 }
 
-// Bits of |x| as fp32 ordered so that infinities and NaNs are the largest.
-template <typename T> __device__ __forceinline__ uint32_t magnitude_bits(T x) {
-    return __float_as_uint((float)x) & 0x7fffffffu;
+// The larger magnitudes of two pairs of 16-bit floats, as bits: those are ordered
+// as the numbers are, with infinities and NaNs the largest.
+__device__ __forceinline__ uint32_t larger_of_pairs(uint32_t most, uint32_t x) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                  __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+}
+// The larger one's bits as fp32.
+template <typename T> __device__ __forceinline__ uint32_t larger_of_pair(uint32_t most) {
+    const unsigned short bits = (unsigned short)max(most & 0xffffu, most >> 16);
+    return __float_as_uint((float)__builtin_bit_cast(T, bits));
 }
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
@@ -263,7 +269,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
     return x;
 }
 
-template <typename T> struct alignas(4) Pair {
+template <typename T> struct Pair {
     T v[2];
 };
 
@@ -294,35 +300,49 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
     const bool active = unit < 2 * p.Hkv;
     const int part = active && unit >= p.Hkv ? 1 : 0;
     const int head = active ? unit - part * p.Hkv : 0;
+    // This lane's first key vector (token, vector of its row) and the step of 64.
+    const int key_tok = lane / (D >> 3), key_col = lane - key_tok * (D >> 3);
+    const int key_step_tok = 64 / (D >> 3), key_step_col = 64 - key_step_tok * (D >> 3);
+    // Its columns and tokens of a value group.
+    const int pairs = DC == 64 ? 32 : 64;
+    const int vcol = 2 * (lane % pairs), vtok = DC == 64 ? 8 * (lane / pairs) : 0;
+    const int vlane = vtok * p.token_stride[1] + vcol;
 
-    // The tokens of this workgroup's slice at which a run begins.
+    // The slots from this workgroup's slice on, one a lane, and where runs begin.
     const int64_t t_begin = (int64_t)blockIdx.x * p.slice;
     const int in_slice = (int)min((int64_t)p.slice, p.tokens - t_begin);
-    auto block_at = [&](int64_t t) {
-        return t >= 0 && t < p.tokens ? block_of_slot(p.slots[t], p.capacity, p.shift) : (int64_t)-1;
-    };
-    const int64_t mine = lane < in_slice ? block_at(t_begin + lane) : -1;
-    int64_t before = __shfl_up((long long)mine, 1, 64);
-    if (lane == 0) before = block_at(t_begin - 1);
-    uint64_t begins = __ballot(mine >= 0 && mine != before);
+    auto slot_at = [&](int64_t t) { return t >= 0 && t < p.tokens ? p.slots[t] : (int64_t)-1; };
+    auto block_of = [&](int64_t slot) { return block_of_slot(slot, p.capacity, p.shift); };
+    const int64_t window = slot_at(t_begin + lane);
+    int64_t before = __shfl_up((long long)window, 1, 64);
+    if (lane == 0) before = slot_at(t_begin - 1);
+    const bool goes_on = block_of(window) >= 0 && block_of(window) == block_of(before);
+    const uint64_t continues = __ballot(goes_on), steps = __ballot(goes_on && window == before + 1);
+    uint64_t begins = __ballot(lane < in_slice && block_of(window) >= 0) & ~continues;
 
     while (begins) {
-        const int64_t t = t_begin + __builtin_ctzll(begins);
+        const int at = __builtin_ctzll(begins);
         begins &= begins - 1;
+        const int64_t t = t_begin + at;
+        const int64_t slot = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(window >> 32), at) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)window, at));
+        const int64_t block = slot >> p.shift;
         // The run's length, and whether its slots are consecutive.
-        const int64_t slot = p.slots[t], block = slot >> p.shift;
-        int length = 0;
-        bool consecutive = true;
-        for (;; length += 64) {
-            const int64_t i = t + length + lane;
-            const int64_t s = i < p.tokens ? p.slots[i] : -1;
-            const bool in = block_of_slot(s, p.capacity, p.shift) == block;
-            const uint64_t out = __ballot(!in), other = __ballot(in && s != slot + length + lane);
-            const int here = out ? __builtin_ctzll(out) : 64;
-            consecutive &= (here == 64 ? other : other & ((1ull << here) - 1)) == 0;
-            if (out) {
-                length += here;
-                break;  // at the call's last token at the latest
+        const uint64_t behind = at < 63 ? ~(continues >> (at + 1)) : ~0ull;
+        int length = 1 + (behind ? __builtin_ctzll(behind) : 63);
+        const uint64_t inside = length > 1 ? (~0ull >> (64 - (length - 1))) << (at + 1) : 0;
+        bool consecutive = (steps & inside) == inside;
+        if (at + length >= 64) {  // it may go on behind the window
+            for (;; length += 64) {
+                const int64_t s = slot_at(t + length + lane);
+                const bool in = block_of(s) == block;
+                const uint64_t out = __ballot(!in), other = __ballot(in && s != slot + length + lane);
+                const int here = out ? __builtin_ctzll(out) : 64;
+                consecutive &= (here == 64 ? other : other & ((1ull << here) - 1)) == 0;
+                if (out) {
+                    length += here;
+                    break;  // at the call's last token at the latest
+                }
             }
         }
         Run run{(int)(slot & (bt - 1)), length, nullptr};
@@ -335,18 +355,21 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
             run.winner = s_winner;
         }
         const bool begun = run.token(0) >= 0;
+        // The group whole, from consecutive tokens: nothing to look up or to keep.
+        const bool whole = consecutive && run.first <= g * 16 && run.first + length >= g * 16 + 16;
 
         const int64_t where = block * p.Hkv + head;
         const float old_scale = active ? p.scales[part][where] : 0.0f;
-        const T* x = (const T*)p.x[part] + t * p.token_stride[part] + head * p.head_stride[part];
-        const int64_t ts = p.token_stride[part];
+        const int ts = p.token_stride[part];
+        const T* x = (const T*)p.x[part] + t * ts + head * p.head_stride[part];
+        const T* rows = x + (int64_t)(g * 16 - run.first) * ts;  // of a whole group
         uint8_t* codes = p.codes[part] + where * bt * D + g * 16 * D;
-        uint32_t most = 0;
         float stored;
 
-        // All of a unit's wavefronts meet here.
-        auto scale_of = [&]() {
-            most = wave_max_u32(most);
+        // The unit's scale from a lane's largest pair.  All of a unit's wavefronts
+        // meet here.
+        auto scale_of = [&](uint32_t pair) {
+            uint32_t most = wave_max_u32(larger_of_pair<T>(pair));
             if (groups > 1) {
                 __syncthreads();  // the run before has read its maxima
                 if (lane == 0) s_max[wave] = most;
@@ -358,34 +381,56 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
 
         if (part == 0) {
             // Keys: vector c of the group is 8 columns of token c / (D/8).
-            Vec16<T> kx[KI];
-            int win[KI];
+            u32x4 kx[KI];
+            uint32_t have = 0, pair = 0;
+            int tok = key_tok, col = key_col;
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
-                const int c = lane + 64 * i, tok = c / (D >> 3), col = 8 * (c - tok * (D >> 3));
-                win[i] = active && tok < 16 ? run.token(g * 16 + tok) : -1;
-                if (win[i] >= 0) kx[i] = *(const Vec16<T>*)(x + win[i] * ts + col);
+                kx[i] = (u32x4){0u, 0u, 0u, 0u};
+                if (tok < 16 && active) {
+                    if (whole) {
+                        kx[i] = *(const u32x4*)(rows + (int64_t)tok * ts + 8 * col);
+                        have |= 1u << i;
+                    } else {
+                        const int w = run.token(g * 16 + tok);
+                        if (w >= 0) {
+                            kx[i] = *(const u32x4*)(x + (int64_t)w * ts + 8 * col);
+                            have |= 1u << i;
+                        }
+                    }
+                }
+                tok += key_step_tok;
+                col += key_step_col;
+                if (col >= D >> 3) {
+                    col -= D >> 3;
+                    ++tok;
+                }
             }
 #pragma unroll
             for (int i = 0; i < KI; ++i)
-                if (win[i] >= 0) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) most = max(most, magnitude_bits(kx[i].v[k]));
-                }
-            const UnitScale u = scale_of();
+                for (int k = 0; k < 4; ++k) pair = larger_of_pairs(pair, kx[i][k]);
+            const UnitScale u = scale_of(pair);
             if (!active) continue;
+            const bool finite = __builtin_amdgcn_readfirstlane(u.finite);
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
                 const int c = lane + 64 * i;
                 if (c >= 2 * D) continue;
                 u32x2* to = (u32x2*)(codes + 8 * c);
                 u32x2 r = {0u, 0u};
-                if (win[i] >= 0) {
-                    float y[8];
+                if (have >> i & 1) {
+                    if (finite) {
+                        float y[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) y[k] = u.finite ? (float)kx[i].v[k] * u.inverse : 0.0f;
-                    r[0] = Code<CT>::pack(y);
-                    r[1] = Code<CT>::pack(y + 4);
+                        for (int k = 0; k < 4; ++k) {
+                            const Pair<T> two = __builtin_bit_cast(Pair<T>, (uint32_t)kx[i][k]);
+                            y[2 * k] = (float)two.v[0] * u.inverse;
+                            y[2 * k + 1] = (float)two.v[1] * u.inverse;
+                        }
+                        r[0] = Code<CT>::pack(y);
+                        r[1] = Code<CT>::pack(y + 4);
+                    }
                 } else if (!begun) {
                     if (u.ratio == 1.0f) continue;
                     r = *to;
@@ -396,28 +441,33 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
             }
         } else {
             // Values: lane (pair, part of the group) holds two columns of NT tokens.
-            const int pairs = DC == 64 ? 32 : 64;
-            const int vcol = 2 * (lane % pairs), vtok = DC == 64 ? 8 * (lane / pairs) : 0;
-            Pair<T> vx[PI][NT];
-            uint32_t have = 0;  // tokens of the call, a bit each
+            uint32_t vx[PI][NT], have = (1u << NT) - 1u, pair = 0;
+            if (whole) {
 #pragma unroll
-            for (int k = 0; k < NT; ++k) {
-                const int w = run.token(g * 16 + vtok + k);
-                if (w >= 0) have |= 1u << k;
+                for (int k = 0; k < NT; ++k)
 #pragma unroll
-                for (int q = 0; q < PI; ++q) {
-                    const int col = vcol + 128 * q;
-                    vx[q][k].v[0] = vx[q][k].v[1] = (T)0.0f;
-                    if (w >= 0 && col < D) vx[q][k] = *(const Pair<T>*)(x + w * ts + col);
+                    for (int q = 0; q < PI; ++q)
+                        vx[q][k] = vcol + 128 * q < D ? *(const uint32_t*)(rows + (int64_t)k * ts + vlane + 128 * q) : 0u;
+            } else {
+                have = 0;
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    const int w = run.token(g * 16 + vtok + k);
+                    if (w >= 0) have |= 1u << k;
+#pragma unroll
+                    for (int q = 0; q < PI; ++q) {
+                        vx[q][k] = 0;
+                        if (w >= 0 && vcol + 128 * q < D)
+                            vx[q][k] = *(const uint32_t*)(x + (int64_t)w * ts + vcol + 128 * q);
+                    }
                 }
             }
 #pragma unroll
             for (int q = 0; q < PI; ++q)
 #pragma unroll
-                for (int k = 0; k < NT; ++k)
-                    most = max(most, max(magnitude_bits(vx[q][k].v[0]), magnitude_bits(vx[q][k].v[1])));
-            const UnitScale u = scale_of();
-            const bool all = have == (1u << NT) - 1u;
+                for (int k = 0; k < NT; ++k) pair = larger_of_pairs(pair, vx[q][k]);
+            const UnitScale u = scale_of(pair);
+            const bool finite = __builtin_amdgcn_readfirstlane(u.finite), all = have == (1u << NT) - 1u;
 #pragma unroll
             for (int q = 0; q < PI; ++q) {
                 const int col = vcol + 128 * q;
@@ -426,13 +476,16 @@ template <typename T, int CT, int DC> __global__ __launch_bounds__(512) void pag
                 for (int e = 0; e < 2; ++e) {
                     typedef uint32_t words __attribute__((ext_vector_type(NT / 4)));
                     words* to = (words*)(codes + (col + e) * 16 + vtok);
-                    words r;
+                    words r = {};
+                    if (finite) {
 #pragma unroll
-                    for (int k4 = 0; k4 < NT / 4; ++k4) {
-                        float y[4];
+                        for (int k4 = 0; k4 < NT / 4; ++k4) {
+                            float y[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = u.finite ? (float)vx[q][4 * k4 + k].v[e] * u.inverse : 0.0f;
-                        r[k4] = Code<CT>::pack(y);
+                            for (int k = 0; k < 4; ++k)
+                                y[k] = (float)__builtin_bit_cast(Pair<T>, vx[q][4 * k4 + k]).v[e] * u.inverse;
+                            r[k4] = Code<CT>::pack(y);
+                        }
                     }
                     if (!all) {
                         if (have == 0 && !begun && u.ratio == 1.0f) continue;
@@ -527,10 +580,13 @@ int kf_paged_cache_append(const void* key, const void* value, const int64_t* slo
     KF_REQUIRE(((uintptr_t)key | (uintptr_t)value | (uintptr_t)key_cache | (uintptr_t)value_cache) % 16 == 0 &&
                    (key_token_stride | key_head_stride | value_token_stride | value_head_stride) % 8 == 0,
                KF_E_INVALID, "kf_paged_cache_append: rows must be aligned to 16 bytes");
+    KF_REQUIRE(key_token_stride >= 0 && key_token_stride < 1 << 26 && value_token_stride >= 0 &&
+                   value_token_stride < 1 << 26,
+               KF_E_UNSUPPORTED, "kf_paged_cache_append: token strides must be below 2^26");
     AppendParams p{{key, value},
                    {(uint8_t*)key_cache, (uint8_t*)value_cache},
                    {key_scale, value_scale},
-                   {key_token_stride, value_token_stride},
+                   {(int)key_token_stride, (int)value_token_stride},
                    {key_head_stride, value_head_stride},
                    slots,
                    tokens,

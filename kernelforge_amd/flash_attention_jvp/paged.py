@@ -117,7 +117,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """t [tokens, heads, D] itself where its rows can be read as 16-byte vectors (a
     part of a packed projection can), else a copy."""
     st, sh, sd = t.stride()
-    if sd == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
+    if sd == 1 and st % 8 == 0 and 0 <= st < 1 << 26 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
