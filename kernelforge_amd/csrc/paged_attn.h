@@ -109,13 +109,12 @@ __device__ __forceinline__ void fill_rows(const PagedParams& p, int from, int to
 }
 
 // Joins the parts of one row and writes it.  LANES threads hold its columns, eight
-// each, and 128 / LANES sets of them take every so-many-th part (place(k) of
-// `to`); the sets meet in LDS.  The order of the additions follows from the
+// each, and WAYS sets of them take every WAYS-th part (place(k) of `from`); the
+// sets meet in LDS.  The order of the additions follows from the
 // lengths alone.  Called by all of a workgroup's 256 threads.
-template <typename T, int LANES, typename Place>
+template <typename T, int LANES, int WAYS, typename Place>
 __device__ __forceinline__ void join_parts(const PagedParams& p, const Partials& from, bool live, int way, int col,
                                            int parts, const Place& place, const Request& r, int head, int row) {
-    constexpr int WAYS = 128 / LANES;
     __shared__ f32x4 s_o[2][256];
     __shared__ float2 s_ml[256];
     const int tid = threadIdx.x;
@@ -137,25 +136,28 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, const Partials&
             m = now;
         }
     }
-    s_o[0][tid] = o0;
-    s_o[1][tid] = o1;
-    s_ml[tid] = make_float2(m, l);
-    __syncthreads();
-    if (!live || way != 0) return;
     float best = m;
+    if constexpr (WAYS > 1) {
+        s_o[0][tid] = o0;
+        s_o[1][tid] = o1;
+        s_ml[tid] = make_float2(m, l);
+        __syncthreads();
+        if (!live || way != 0) return;
 #pragma unroll
-    for (int k = 1; k < WAYS; ++k) best = fmaxf(best, s_ml[tid + k * LANES].x);
-    const float base = best == -__builtin_inff() ? 0.0f : best;
-    l = 0.0f;
-    o0 = o1 = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 1; k < WAYS; ++k) best = fmaxf(best, s_ml[tid + k * LANES].x);
+        const float base = best == -__builtin_inff() ? 0.0f : best;
+        l = 0.0f;
+        o0 = o1 = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < WAYS; ++k) {
-        const float2 one = s_ml[tid + k * LANES];
-        const float f = __builtin_amdgcn_exp2f(one.x - base);
-        l += one.y * f;
-        o0 += s_o[0][tid + k * LANES] * f;
-        o1 += s_o[1][tid + k * LANES] * f;
+        for (int k = 0; k < WAYS; ++k) {
+            const float2 one = s_ml[tid + k * LANES];
+            const float f = __builtin_amdgcn_exp2f(one.x - base);
+            l += one.y * f;
+            o0 += s_o[0][tid + k * LANES] * f;
+            o1 += s_o[1][tid + k * LANES] * f;
+        }
     }
+    if (!live) return;
     const int i = row / p.G, token = r.q0 + i, h = head * p.G + row % p.G;
     const bool none = reach(p, r, i) <= 0;
     Vec16<T> v;

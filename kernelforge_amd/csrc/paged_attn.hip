@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p, Shares w
     const Request r{whole.q0, whole.n, whole.ctx};
     const int row = whole.row_tile * unit_rows + x;
     const bool live = row < min(r.n, p.max_q) * p.G && col < p.D;
-    join_parts<T, LANES>(
+    join_parts<T, LANES, WAYS>(
         p, w.to, live, way, col, whole.parts,
         [&](int k) { return (int64_t)(k == 0 ? whole.part : 2 * ((int)blockIdx.x + k)) * unit_rows + x; }, r,
         whole.head, row);

@@ -598,9 +598,8 @@ int kf_paged_cache_append(const void* key, const void* value, const int64_t* slo
     const int groups = 1 << (shift - 4), waves = groups > 4 ? groups : 4;
     const int64_t gy = (2 * Hkv * groups + waves - 1) / waves;
     // Decoding gives every token a block of its own: a workgroup each.  Prompts
-    // start a run every block_tokens tokens: a workgroup for as many (64 at most,
-    // the lanes that look for a run's start).
-    p.slice = tokens * gy <= 4096 ? 1 : shift < 6 ? 1 << shift : 64;
+    // begin a run every block_tokens tokens: a workgroup for 16.
+    p.slice = tokens * gy <= 4096 ? 1 : 16;
     const int64_t gx = (tokens + p.slice - 1) / p.slice;
     const dim3 grid((unsigned)gx, (unsigned)gy);
     const hipStream_t s = (hipStream_t)stream;

@@ -174,9 +174,11 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
     auto scales_of = [&](int tile, int block) {
         const int64_t at = (int64_t)max(block, 0) * p.Hkv + head;
         const float vs = uniform_load(p.vs + at);
-        float2 s = make_float2(uniform_load(p.ks + at) * p.c, vs < __builtin_inff() ? vs : __builtin_nanf(""));
+        // A key scale of 0 is held above it, so that a hidden key's -inf stays one.
+        const float ks = uniform_load(p.ks + at) * p.c;
+        float2 s = make_float2(ks < kLeastScale ? kLeastScale : ks, vs < __builtin_inff() ? vs : __builtin_nanf(""));
         if (block < 0) s = make_float2(__builtin_nanf(""), 0.0f);
-        if (64 * tile + 16 * wave >= r.ctx) s = make_float2(0.0f, 0.0f);  // says nothing
+        if (64 * tile + 16 * wave >= r.ctx) s = make_float2(1.0f, 0.0f);  // says nothing
         return s;
     };
 
@@ -261,29 +263,26 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
             }
             const int key0 = 64 * tile + 16 * quarter;  // position of this lane's first key
             const bool edge = 64 * tile + 64 > all_see;
+            // The lane's keys share a scale, which is not negative: their largest
+            // product is their largest score.
             float most[RT];
             bool rise = false;
-            auto scale_scores = [&](auto at_edge) {
+            auto hide = [&](int rt, int t, int i) { return key0 + 4 * t + i >= limit[rt]; };
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    most[rt] = -__builtin_inff();
+            for (int rt = 0; rt < RT; ++rt) {
+                if (edge) {
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float x = s[rt][t][i] * mine.x;
-                            if (decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt]) x = -__builtin_inff();
-                            s[rt][t][i] = x;
-                            most[rt] = fmaxf(most[rt], x);
-                        }
-                    most[rt] = row_max4(most[rt]);
-                    rise |= most[rt] > ref[rt] + kRise;
+                        for (int i = 0; i < 4; ++i)
+                            if (hide(rt, t, i)) s[rt][t][i] = -__builtin_inff();
                 }
-            };
-            if (edge)
-                scale_scores(std::true_type());
-            else
-                scale_scores(std::false_type());
+                float x = s[rt][0][0];
+#pragma unroll
+                for (int k = 1; k < 16; ++k) x = fmaxf(x, s[rt][k >> 2][k & 3]);
+                most[rt] = row_max4(x * mine.x);
+                rise |= most[rt] > ref[rt] + kRise;
+            }
             // The references follow the rows' maxima when one has risen by 2^kRise.
             if (__any(rise) || vmax > vref) {
                 const float shrink = vmax > vref ? vref / vmax : 1.0f;
@@ -301,29 +300,29 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
                     for (int d = 0; d < VT; ++d) acc[rt][d] *= alpha * shrink;
                 }
             }
+            // exp2(score - reference) * factor as one exponential of one fma; the
+            // sum takes the factor out again.  A factor below 2^-60 counts as 2^-60:
+            // its products are 0 in f16 either way.
             const float factor = mine.y * inv_vref * kPromptPScale;
+            const float least = factor < 0x1p-60f ? 0x1p-60f : factor;  // keeps a NaN
+            const float lift = __builtin_amdgcn_logf(least), unlift = __builtin_amdgcn_exp2f(-lift);
             V<f16>::x8 pf[RT][2];
-            auto probabilities = [&](auto at_edge) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const float base = ref[rt] == -__builtin_inff() ? 0.0f : ref[rt];
+            for (int rt = 0; rt < RT; ++rt) {
+                const float base = lift - (ref[rt] == -__builtin_inff() ? 0.0f : ref[rt]);
+                float add = 0.0f;
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float e = __builtin_amdgcn_exp2f(s[rt][t][i] - base);
-                            sum[rt] += e;
-                            // A hidden key's weight is 0 whatever its block's scale.
-                            const float x =
-                                decltype(at_edge)::value && key0 + 4 * t + i >= limit[rt] ? 0.0f : e * factor;
-                            pf[rt][t >> 1][4 * (t & 1) + i] = (f16)x;
-                        }
-                }
-            };
-            if (edge)
-                probabilities(std::true_type());
-            else
-                probabilities(std::false_type());
+                    for (int i = 0; i < 4; ++i) {
+                        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], mine.x, base));
+                        // A hidden key's weight is 0 whatever its block's scale.
+                        if (edge && hide(rt, t, i)) e = 0.0f;
+                        add += e;
+                        pf[rt][t >> 1][4 * (t & 1) + i] = (f16)e;
+                    }
+                sum[rt] += add == 0.0f ? 0.0f : add * unlift;  // rows that see no key of a NaN scale
+            }
 #pragma unroll
             for (int d = 0; d < VT; ++d) {
                 const u32x4 v = *(const u32x4*)(values + read_v + 256 * d + (d & 1 ? -swap : swap));
@@ -368,18 +367,16 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
     }
 }
 
-// Joins a unit's splits, in order: two rows a workgroup, LANES threads with eight
-// columns each a row, WAYS sets of them that take every WAYS-th split.
+// Joins a unit's splits, in order: LANES threads with eight columns each a row.
 template <typename T, int ROWS, int LANES>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedParams p, PromptWork w) {
-    constexpr int WAYS = 128 / LANES;
     const Unit u = unit_at<ROWS>(p, w.units - 1 - blockIdx.x);
     if (u.b < 0) return;
-    const int tid = threadIdx.x, col = 8 * (tid % LANES), way = tid / LANES % WAYS;
-    const int x = blockIdx.y * 2 + tid / 128, row = u.row0 + x;
+    const int tid = threadIdx.x, col = 8 * (tid % LANES);
+    const int x = blockIdx.y * (256 / LANES) + tid / LANES, row = u.row0 + x;
     const bool live = row < min(u.r.n, p.max_q) * p.G && col < p.D;
-    join_parts<T, LANES>(
-        p, w.to, live, way, col, w.splits,
+    join_parts<T, LANES, 1>(
+        p, w.to, live, 0, col, w.splits,
         [&](int k) { return ((int64_t)blockIdx.x * w.splits + k) * ROWS + x; }, u.r, u.head, row);
 }
 
@@ -389,7 +386,7 @@ int launch_shape(const PagedParams& p, const PromptWork& w, hipStream_t s) {
     paged_prompt_kernel<T, CT, DP><<<dim3((unsigned)w.units, (unsigned)w.splits), 256, 0, s>>>(p, w);
     int rc = check_launch("kf_paged_attention (prompts)");
     if (rc != KF_OK || w.splits == 1) return rc;
-    paged_prompt_join_kernel<T, ROWS, DP / 8><<<dim3((unsigned)w.units, ROWS / 2), 256, 0, s>>>(p, w);
+    paged_prompt_join_kernel<T, ROWS, DP / 8><<<dim3((unsigned)w.units, ROWS * (DP / 8) / 256), 256, 0, s>>>(p, w);
     return check_launch("kf_paged_attention (prompts' join)");
 }
 
