@@ -16,34 +16,34 @@ constexpr float kRise = 3.0f;
 // The products and their operand layouts are those of the few-rows kernel
 // (paged_attn.hip): S^T = K Q^T leaves each lane the scores of one 16-token
 // group, which are the second product's operand as they are.  Here all
-// wavefronts read the same keys, so the codes go through LDS, as codes: half
-// the LDS traffic of 16-bit elements, which at 32 rows a wavefront keeps the
-// reads at half of what the LDS delivers while the matrix cores run.  Each
-// wavefront copies one of the tile's four groups (global_load_lds, 16 bytes a
-// lane), whose block, address and scales are then scalars; a tile is copied
-// while the one before it is used, with one barrier a tile.
+// wavefronts read the same keys.  Each loads the codes of one of a tile's four
+// groups, whose block, address and scales are scalars, a tile ahead into
+// registers, and writes them into LDS as 16-bit floats behind the first product
+// of the tile before; one barrier a tile.
 //
-// Keys lie in LDS as rows of DP bytes whose 16-byte chunks are permuted by
-// key_swizzle, values as the cache holds them except that odd groups have each
-// pair of 16-column tiles exchanged; both leave the 16-byte operand reads
-// without bank conflicts in 32-lane passes over 128 banks.
+// Issue-bound (counters: the SIMDs issue in 83% of the cycles, two wavefronts
+// each), so what counts is the instructions for a key: codes that every
+// wavefront converted for itself, behind LDS tiles of codes, ran XX.
+//
+// Keys lie in LDS as rows of 16-byte chunks (8 elements) permuted by key_swizzle,
+// values as [group][column][16 tokens] with the halves of odd groups exchanged;
+// both leave the operand reads without bank conflicts in 32-lane passes over
+// 128 banks.
 // ---------------------------------------------------------------------------
 template <int DP> struct PromptShape {
-    static constexpr int RT = DP > 128 ? 1 : 2;
-    static constexpr int ROWS = 64 * RT;  // of a workgroup
+    static constexpr int WAVES = 8;
+    static constexpr int ROWS = 16 * WAVES;            // of a workgroup
+    static constexpr int CH = DP == 96 ? 16 : DP / 8;  // 16-byte chunks of a key row in LDS
+    static constexpr int BUFFERS = DP > 128 ? 1 : 2;   // two workgroups share a CU's LDS
+    static constexpr int OCC = DP > 128 ? 2 : 4;       // wavefronts a SIMD
 };
 
-// The permutation of a key row's 16-byte chunks.
-template <int DP> __device__ __forceinline__ int key_swizzle(int key) {
+// The permutation of a key row's chunks.
+template <int CH> __device__ __forceinline__ int key_swizzle(int key) {
     const int g = (key >> 4) & 3, e = key & 3;
-    if constexpr (DP == 64) return g;
-    else if constexpr (DP == 128) return 2 * g + (e >> 1);
-    else return 2 * g + 8 * (e >> 1) + (e & 1);
-}
-// The row of LDS that holds a key: with four chunks a row, odd groups exchange
-// rows 4 apart, which puts them in the other half of the banks.
-template <int DP> __device__ __forceinline__ int key_row(int key) {
-    return DP == 64 ? key ^ (((key >> 4) & 1) << 2) : key;
+    if constexpr (CH == 8) return 2 * g + (e >> 1);
+    else if constexpr (CH == 16) return 2 * g + 8 * (e >> 1) + (e & 1);
+    else return 2 * (4 * g + e);
 }
 
 // Integers and scales that one wavefront's lanes share, through scalar loads.
@@ -68,16 +68,16 @@ template <int ROWS> __device__ __forceinline__ Unit unit_at(const PagedParams& p
     u.head = unit % p.Hkv;
     const int index = unit / p.Hkv;
     auto tile_of = [&](int first, int b) { return (int)(((int64_t)first * p.G) / ROWS) + b; };
+    // The last request whose tiles begin at or before this one, by 64ths.
     int b = 0;
-    for (int lo = 0, hi = p.B; lo < hi;) {
-        const int mid = (lo + hi) >> 1;
-        const int first = p.starts ? clamp_int(uniform_load(p.starts + mid), 0, p.tokens) : mid;
-        if (tile_of(first, mid) <= index) {
-            b = mid;
-            lo = mid + 1;
-        } else {
-            hi = mid;
-        }
+    for (int count = p.B; count > 1;) {
+        const int step = (count + 63) >> 6, at = b + step * (int)(threadIdx.x & 63);
+        const bool in = at < b + count;
+        const int first = !in ? 0 : p.starts ? clamp_int(p.starts[at], 0, p.tokens) : at;
+        const int before = __builtin_popcountll(__ballot(in && tile_of(first, at) <= index));
+        const int skip = step * (before > 0 ? before - 1 : 0);
+        b += skip;
+        count = min(count - skip, step);
     }
     u.b = __builtin_amdgcn_readfirstlane(b);
     u.r = uniform_request(p, u.b);
@@ -88,16 +88,18 @@ template <int ROWS> __device__ __forceinline__ Unit unit_at(const PagedParams& p
 }
 
 template <typename T, int CT, int DP>
-__global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, PromptWork w) {
-    constexpr int RT = PromptShape<DP>::RT, ROWS = PromptShape<DP>::ROWS;
-    constexpr int KC = DP / 64, VT = DP / 16, CH = DP / 16;
-    constexpr int TILE = 64 * DP;  // bytes of a tile's keys or values
-    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][TILE];
-    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][TILE];
-    __shared__ float2 s_scales[2][4];  // key scale (NaN: no such block), value scale
+__global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) void paged_prompt_kernel(PagedParams p, PromptWork w) {
+    using Shape = PromptShape<DP>;
+    constexpr int RT = 1, ROWS = Shape::ROWS, CH = Shape::CH, BUFFERS = Shape::BUFFERS;
+    constexpr int KC = DP / 32, VT = DP / 16;
+    constexpr int NC = (DP + 127) / 128;  // 16-byte vectors of half a group's codes a lane
+    __shared__ u32x4 s_keys[BUFFERS][64 * CH];
+    __shared__ u32x4 s_values[BUFFERS][64 * DP / 8];
+    __shared__ float2 s_scales[BUFFERS][4];  // key scale (NaN: no such block), value scale
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, quarter = lane >> 4;
+    const int group = wave >> 1;  // of a tile, this wavefront's and its neighbour's
     const int D = p.D;
 
     // The latest units, which see the most keys, go first.
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
     // This wavefront's rows.
     const int my_row0 = row0 + 16 * RT * wave;
     int limit[RT];
-    typename V<T>::x8 qf[RT][KC][2];
+    typename V<T>::x8 qf[RT][KC];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = my_row0 + 16 * rt + m, i = row / p.G;
@@ -119,57 +121,80 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
         limit[rt] = live ? reach(p, r, i) : 0;
         const T* q = (const T*)p.q + (int64_t)(r.q0 + i) * p.q_ts + (int64_t)(head * p.G + row % p.G) * p.q_hs;
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int col = 64 * c + 16 * quarter + 8 * h;
-                u32x4 v = {0u, 0u, 0u, 0u};
-                if (live && col < D) v = *(const u32x4*)(q + col);
-                qf[rt][c][h] = __builtin_bit_cast(typename V<T>::x8, v);
-            }
+        for (int c = 0; c < KC; ++c) {
+            const int col = 32 * c + 8 * quarter;
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (live && col < D) v = *(const u32x4*)(q + col);
+            qf[rt][c] = __builtin_bit_cast(typename V<T>::x8, v);
+        }
     }
     auto seen_by = [&](int row) {
         return __builtin_amdgcn_readfirstlane(keys_to_scan(p, reach(p, r, min(row, rows - 1) / p.G)));
     };
-    // Keys that the wavefront's rows all see, and that any sees.
+    // Keys that the wavefront's rows all see.
     const int all_see = my_row0 < rows ? __builtin_amdgcn_readfirstlane(reach(p, r, my_row0 / p.G)) : 0;
-    const int any_sees = my_row0 < rows ? seen_by(my_row0 + 16 * RT - 1) : 0;
     const int tiles = (seen_by(row0 + ROWS - 1) + 63) >> 6;
     const int first = (int)((int64_t)tiles * blockIdx.y / w.splits);
     const int last = (int)((int64_t)tiles * (blockIdx.y + 1) / w.splits);
 
-    // Copies of this wavefront's group.  Lane i of instruction j fills the group's
-    // 16-byte slot 64 j + i.
+    // This wavefront's group: a lane's vectors of codes and where they go.
     const int subs = (1 << (p.shift - 4)) - 1;
     const int64_t unit_bytes = (int64_t)D << p.shift;
-    uint32_t from_k[DP / 64], from_v[DP / 64];
+    // The codes of a group lie as they are read; past D the query is 0 and columns
+    // are not written, so any bytes of the group serve there.
+    uint32_t from_k[NC], from_v[NC], to_k[NC];
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
-        const int slot = 64 * j + lane;
-        const int key = key_row<DP>(16 * wave + slot / CH);  // an exchange is its own inverse
-        const int chunk = (slot % CH) ^ key_swizzle<DP>(key);
-        from_k[j] = (key & 15) * D + (16 * chunk < D ? 16 * chunk : 0);  // past D: any bytes, the query is 0 there
-        const int col = slot ^ ((wave & 1) << 4);
-        from_v[j] = 16 * (col < D ? col : 0);  // past D: columns that are not written
+    for (int j = 0; j < NC; ++j) {
+        const int slot = (wave & 1) * (DP / 2) + 64 * j + lane, key = slot / (DP / 16), chunk = slot % (DP / 16);
+        from_k[j] = key < 16 ? key * D + (16 * chunk < D ? 16 * chunk : 0) : 0;
+        from_v[j] = slot < D ? 16 * slot : 0;
+        if (DP / 2 % 64 != 0 && slot >= DP) from_k[j] = from_v[j] = 0;
+        to_k[j] = (16 * group + key) * CH + ((2 * chunk) ^ key_swizzle<CH>(16 * group + key));  // the other half's ^ 1
     }
+    const uint32_t to_v = (group * DP + (wave & 1) * (DP / 2) + lane) * 2 + (group & 1);  // likewise
     const int* table = p.tables + (int64_t)b * p.width;
     auto entry_of = [&](int tile) {
-        const int entry = (4 * tile + wave) >> (p.shift - 4);
+        const int entry = (4 * tile + group) >> (p.shift - 4);
         return uniform_load(table + min(entry, p.width - 1));
     };
     auto block_of = [&](int id, int tile) {
-        return __builtin_amdgcn_readfirstlane(block_of_entry(id, p.width, p.blocks, p.shift, 4 * tile + wave));
+        return __builtin_amdgcn_readfirstlane(block_of_entry(id, p.width, p.blocks, p.shift, 4 * tile + group));
     };
-    const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_addr(&s_keys[0][0])) + wave * 16 * DP;
-    const uint32_t lds_v = __builtin_amdgcn_readfirstlane(lds_addr(&s_values[0][0])) + wave * 16 * DP;
-    auto copy_tile = [&](int tile, int block) {
-        const int64_t at = ((int64_t)max(block, 0) * p.Hkv + head) * unit_bytes + 16 * ((4 * tile + wave) & subs) * D;
-        const uint32_t buffer = (tile & 1) * TILE;
+    u32x4 codes_k[NC], codes_v[NC];
+    auto load_codes = [&](int tile, int block) {
+        const int64_t at = ((int64_t)max(block, 0) * p.Hkv + head) * unit_bytes + 16 * ((4 * tile + group) & subs) * D;
+        const uint8_t *k = p.kc + at, *v = p.vc + at;
 #pragma unroll
-        for (int j = 0; j < DP / 64; ++j) {
-            lds_copy16_sbase(p.kc + at, from_k[j], lds_k + buffer + 1024 * j);
-            lds_copy16_sbase(p.vc + at, from_v[j], lds_v + buffer + 1024 * j);
+        for (int j = 0; j < NC; ++j) {
+            codes_k[j] = *(const u32x4*)(k + from_k[j]);
+            codes_v[j] = *(const u32x4*)(v + from_v[j]);
         }
+    };
+    auto store_codes = [&](int buffer, int valid) {
+        // Values behind the context or of no block are zeroed: what lies there may be NaN.
+        if (valid < 16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int bytes = clamp_int(valid - 4 * e, 0, 4);
+                const uint32_t mask = bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1u;
+#pragma unroll
+                for (int j = 0; j < NC; ++j) codes_v[j][e] &= mask;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            if (DP / 2 % 64 != 0 && 64 * j + lane >= DP / 2) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const auto k = Codes<T, CT>::x8(codes_k[j][2 * h], codes_k[j][2 * h + 1]);
+                const auto v = Codes<f16, CT>::x8(codes_v[j][2 * h], codes_v[j][2 * h + 1]);
+                s_keys[buffer][to_k[j] ^ h] = __builtin_bit_cast(u32x4, k);
+                s_values[buffer][(to_v + 128 * j) ^ h] = __builtin_bit_cast(u32x4, v);
+            }
+        }
+    };
+    auto valid_of = [&](int tile, int block) {
+        return block < 0 ? 0 : clamp_int(r.ctx - (64 * tile + 16 * group), 0, 16);
     };
     auto scales_of = [&](int tile, int block) {
         const int64_t at = (int64_t)max(block, 0) * p.Hkv + head;
@@ -178,7 +203,7 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
         const float ks = uniform_load(p.ks + at) * p.c;
         float2 s = make_float2(ks < kLeastScale ? kLeastScale : ks, vs < __builtin_inff() ? vs : __builtin_nanf(""));
         if (block < 0) s = make_float2(__builtin_nanf(""), 0.0f);
-        if (64 * tile + 16 * wave >= r.ctx) s = make_float2(1.0f, 0.0f);  // says nothing
+        if (64 * tile + 16 * group >= r.ctx) s = make_float2(1.0f, 0.0f);  // says nothing
         return s;
     };
 
@@ -191,91 +216,73 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
 #pragma unroll
         for (int d = 0; d < VT; ++d) acc[rt][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // Operand reads: a lane's chunk of column block c, and its values of the even
-    // and of the odd column tiles.
-    uint32_t read_k[KC];
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-        const int key = 16 * (m >> 2) + (m & 3);
-        read_k[c] = key * DP + 16 * ((4 * c + quarter) ^ key_swizzle<DP>(key));
-    }
-    const int exchange = DP == 64 ? ((m >> 2) & 1) << 2 : 0;  // of the rows 4t of odd groups
-    const uint32_t read_v = quarter * 16 * DP + 16 * m;
-    const int swap = (quarter & 1) << 8;
+    // Operand reads: a lane's chunk of column block c, and its values' halves.
+    uint32_t read_k = (16 * (m >> 2) + (m & 3)) * CH + (quarter ^ key_swizzle<CH>(16 * (m >> 2) + (m & 3)));
+    const uint32_t read_v = (quarter * DP + m) * 2 + (quarter & 1);
 
     int block = -1, ahead = 0;
     if (first < last) {
         block = block_of(entry_of(first), first);
-        copy_tile(first, block);
+        load_codes(first, block);
         ahead = entry_of(min(first + 1, last - 1));
         const float2 s = scales_of(first, block);
-        if (lane == 0) s_scales[first & 1][wave] = s;
+        store_codes(0, valid_of(first, block));
+        if (lane == 0) s_scales[0][group] = s;
+        block = block_of(ahead, min(first + 1, last - 1));
+        load_codes(min(first + 1, last - 1), block);
     }
+    int now = 0;
     for (int tile = first; tile < last; ++tile) {
-        const int now = tile & 1;
-        wait_vmem();  // this wavefront's group has arrived
-        {
-            // Values behind the context or of no block are zeroed: what lies there may be NaN.
-            const int valid = block < 0 ? 0 : clamp_int(r.ctx - (64 * tile + 16 * wave), 0, 16);
-            if (valid < 16) {
-#pragma unroll
-                for (int j = 0; j < DP / 64; ++j) {
-                    u32x4* at = (u32x4*)&s_values[now][wave * 16 * DP + 16 * (64 * j + lane)];
-                    u32x4 v = *at;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int bytes = clamp_int(valid - 4 * e, 0, 4);
-                        v[e] &= bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1u;
-                    }
-                    *at = v;
-                }
-            }
-        }
         __syncthreads();
-        float2 next_scales = make_float2(0.0f, 0.0f);
-        if (tile + 1 < last) {
-            block = block_of(ahead, tile + 1);
-            copy_tile(tile + 1, block);
-            ahead = entry_of(min(tile + 2, last - 1));
-            next_scales = scales_of(tile + 1, block);
-        }
-        if (64 * tile < any_sees) {
-            const uint8_t* keys = s_keys[now];
-            const uint8_t* values = s_values[now];
-            const float2 mine = s_scales[now][quarter];
-            float vmax = fmaxf(fmaxf(s_scales[now][0].y, s_scales[now][1].y),
-                               fmaxf(s_scales[now][2].y, s_scales[now][3].y));
-            f32x4 s[RT][4];
+        const int then = min(tile + 1, last - 1);  // the tile in the registers, the last one again at the end
+        const float2 next_scales = scales_of(then, block);
+        auto pass_on = [&](int buffer) {
+            store_codes(buffer, valid_of(then, block));
+            if (lane == 0) s_scales[buffer][group] = next_scales;
+            const int after = min(tile + 2, last - 1);
+            block = block_of(entry_of(after), after);
+            load_codes(after, block);
+        };
+        const float2 mine = s_scales[now][quarter];
+        const float vmax = fmaxf(fmaxf(s_scales[now][0].y, s_scales[now][1].y),
+                                 fmaxf(s_scales[now][2].y, s_scales[now][3].y));
+        asm volatile("" : "+v"(read_k));  // its columns' addresses are formed here, not kept
+        f32x4 s[RT][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const u32x4 k = *(const u32x4*)(keys + read_k[c] + ((4 * t) ^ exchange) * DP);
+            for (int c = 0; c < KC; ++c) {
+                const auto a = __builtin_bit_cast(typename V<T>::x8, s_keys[now][(read_k ^ (4 * c)) + 4 * t * CH]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const auto a = Codes<T, CT>::x8(k[2 * h], k[2 * h + 1]);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c][h], s[rt][t]);
-                    }
-                }
+                for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c], s[rt][t]);
             }
-            const int key0 = 64 * tile + 16 * quarter;  // position of this lane's first key
-            const bool edge = 64 * tile + 64 > all_see;
-            // The lane's keys share a scale, which is not negative: their largest
-            // product is their largest score.
-            float most[RT];
-            bool rise = false;
-            auto hide = [&](int rt, int t, int i) { return key0 + 4 * t + i >= limit[rt]; };
+        }
+        if constexpr (BUFFERS == 2) pass_on(now ^ 1);
+        const int key0 = 64 * tile + 16 * quarter;  // position of this lane's first key
+        const bool edge = 64 * tile + 64 > all_see;
+        // The lane's keys share a scale, which is not negative: their largest
+        // product is their largest score.
+        float most[RT];
+        bool rise = false;
+        // Keys of this lane's group that a row sees.  The empty asm keeps the
+        // comparisons out of the tiles that every row sees whole.
+        auto seen_here = [&](int rt) {
+            int n = limit[rt] - key0;
+            asm volatile("" : "+v"(n));
+            return n;
+        };
+        auto largest = [&](auto at_edge) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                if (edge) {
+                if (decltype(at_edge)::value) {
+                    const int n = seen_here(rt);
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (hide(rt, t, i)) s[rt][t][i] = -__builtin_inff();
+                            if (4 * t + i >= n) s[rt][t][i] = -__builtin_inff();
                 }
                 float x = s[rt][0][0];
 #pragma unroll
@@ -283,58 +290,72 @@ __global__ __launch_bounds__(256, 2) void paged_prompt_kernel(PagedParams p, Pro
                 most[rt] = row_max4(x * mine.x);
                 rise |= most[rt] > ref[rt] + kRise;
             }
-            // The references follow the rows' maxima when one has risen by 2^kRise.
-            if (__any(rise) || vmax > vref) {
-                const float shrink = vmax > vref ? vref / vmax : 1.0f;
-                if (vmax > vref) {
-                    vref = vmax;
-                    inv_vref = 1.0f / vmax;
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const float to = fmaxf(ref[rt], most[rt]);
-                    const float alpha = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
-                    ref[rt] = to;
-                    sum[rt] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < VT; ++d) acc[rt][d] *= alpha * shrink;
-                }
+        };
+        if (edge)
+            largest(std::true_type());
+        else
+            largest(std::false_type());
+        // The references follow the rows' maxima when one has risen by 2^kRise.
+        if (__any(rise) || vmax > vref) {
+            const float shrink = vmax > vref ? vref / vmax : 1.0f;
+            if (vmax > vref) {
+                vref = vmax;
+                inv_vref = 1.0f / vmax;
             }
-            // exp2(score - reference) * factor as one exponential of one fma; the
-            // sum takes the factor out again.  A factor below 2^-60 counts as 2^-60:
-            // its products are 0 in f16 either way.
-            const float factor = mine.y * inv_vref * kPromptPScale;
-            const float least = factor < 0x1p-60f ? 0x1p-60f : factor;  // keeps a NaN
-            const float lift = __builtin_amdgcn_logf(least), unlift = __builtin_amdgcn_exp2f(-lift);
-            V<f16>::x8 pf[RT][2];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float to = fmaxf(ref[rt], most[rt]);
+                const float alpha = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
+                ref[rt] = to;
+                sum[rt] *= alpha;
+#pragma unroll
+                for (int d = 0; d < VT; ++d) acc[rt][d] *= alpha * shrink;
+            }
+        }
+        // exp2(score - reference) * factor as one exponential of one fma; the
+        // sum takes the factor out again.  A factor below 2^-60 counts as 2^-60:
+        // its products are 0 in f16 either way.
+        const float factor = mine.y * inv_vref * kPromptPScale;
+        const float least = factor < 0x1p-60f ? 0x1p-60f : factor;  // keeps a NaN
+        const float lift = __builtin_amdgcn_logf(least), unlift = __builtin_amdgcn_exp2f(-lift);
+        V<f16>::x8 pf[RT][2];
+        auto probabilities = [&](auto at_edge) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const float base = lift - (ref[rt] == -__builtin_inff() ? 0.0f : ref[rt]);
                 float add = 0.0f;
+                const int n = decltype(at_edge)::value ? seen_here(rt) : 0;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], mine.x, base));
                         // A hidden key's weight is 0 whatever its block's scale.
-                        if (edge && hide(rt, t, i)) e = 0.0f;
+                        if (decltype(at_edge)::value && 4 * t + i >= n) e = 0.0f;
                         add += e;
                         pf[rt][t >> 1][4 * (t & 1) + i] = (f16)e;
                     }
                 sum[rt] += add == 0.0f ? 0.0f : add * unlift;  // rows that see no key of a NaN scale
             }
+        };
+        if (edge)
+            probabilities(std::true_type());
+        else
+            probabilities(std::false_type());
 #pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                const u32x4 v = *(const u32x4*)(values + read_v + 256 * d + (d & 1 ? -swap : swap));
+        for (int d = 0; d < VT; ++d)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const auto a = Codes<f16, CT>::x8(v[2 * h], v[2 * h + 1]);
+            for (int h = 0; h < 2; ++h) {
+                const auto a = __builtin_bit_cast(V<f16>::x8, s_values[now][(read_v ^ h) + 32 * d]);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
-                }
+                for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
             }
+        if constexpr (BUFFERS == 1) {
+            __syncthreads();
+            pass_on(0);
+        } else {
+            now ^= 1;
         }
-        if (tile + 1 < last && lane == 0) s_scales[now ^ 1][wave] = next_scales;
     }
 
 #pragma unroll
@@ -383,26 +404,29 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedParams p, P
 template <typename T, int CT, int DP>
 int launch_shape(const PagedParams& p, const PromptWork& w, hipStream_t s) {
     constexpr int ROWS = PromptShape<DP>::ROWS;
-    paged_prompt_kernel<T, CT, DP><<<dim3((unsigned)w.units, (unsigned)w.splits), 256, 0, s>>>(p, w);
+    const dim3 grid((unsigned)w.units, (unsigned)w.splits), threads(64 * PromptShape<DP>::WAVES);
+    paged_prompt_kernel<T, CT, DP><<<grid, threads, 0, s>>>(p, w);
     int rc = check_launch("kf_paged_attention (prompts)");
     if (rc != KF_OK || w.splits == 1) return rc;
-    paged_prompt_join_kernel<T, ROWS, DP / 8><<<dim3((unsigned)w.units, ROWS * (DP / 8) / 256), 256, 0, s>>>(p, w);
+    constexpr int LANES = DP == 96 ? 16 : DP / 8;  // of a row's columns
+    paged_prompt_join_kernel<T, ROWS, LANES><<<dim3((unsigned)w.units, ROWS * LANES / 256), 256, 0, s>>>(p, w);
     return check_launch("kf_paged_attention (prompts' join)");
 }
 
 template <typename T, int CT> int launch_dim(const PagedParams& p, const PromptWork& w, hipStream_t s) {
     if (p.D <= 64) return launch_shape<T, CT, 64>(p, w, s);
+    if (p.D <= 96) return launch_shape<T, CT, 96>(p, w, s);
     if (p.D <= 128) return launch_shape<T, CT, 128>(p, w, s);
     return launch_shape<T, CT, 256>(p, w, s);
 }
 
-int unit_rows(int64_t D) { return D > 128 ? PromptShape<256>::ROWS : PromptShape<128>::ROWS; }
+constexpr int kUnitRows = PromptShape<128>::ROWS;
 
 }  // namespace
 
 PromptPlan prompt_plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_ctx) {
     PromptPlan w;
-    const int rows = unit_rows(D);
+    const int64_t rows = kUnitRows;
     w.units = (tokens * (Hq / Hkv) / rows + B) * Hkv;
     // Two workgroups a CU fit; fewer units than CUs have their keys split.
     int64_t splits = w.units >= device_cu_count() ? 1 : (2 * device_cu_count() + w.units - 1) / w.units;
@@ -417,7 +441,7 @@ int launch_prompt(const PagedParams& p, const PromptPlan& plan, void* workspace,
                   hipStream_t stream) {
     PromptWork w;
     w.to.o = (float*)workspace;
-    w.to.ml = (float2*)(w.to.o + plan.units * plan.splits * unit_rows(p.D) * p.D);
+    w.to.ml = (float2*)(w.to.o + plan.units * plan.splits * kUnitRows * p.D);
     w.units = (int)plan.units;
     w.splits = plan.splits;
     const bool e4m3 = cache_dtype == KF_CACHE_E4M3;
