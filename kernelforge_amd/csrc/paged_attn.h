@@ -60,7 +60,6 @@ namespace {
 
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
 
-
 __device__ __forceinline__ Request request(const PagedParams& p, int b) {
     return request_at(p.starts, p.context, b, p.tokens);
 }

@@ -127,20 +127,28 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
     const int m = lane & 15, quarter = lane >> 4;
     const int D = EXACT ? DP : p.D;
 
-    // This workgroup's share of the line.
+    // This workgroup's share of the line.  Where no unit is cut and every request
+    // has one token, all have the same number of units and a unit's request follows
+    // by a division; else every workgroup sums over the requests.
+    const bool uniform = w.aligned && !p.starts;
+    const int units_each = steps_and_units<KEYS, ROWS>(p, Request{0, 1, 0}, true).y;
     const int per = (p.B + 255) / 256;
     const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
     // A thread's first request, most often its only one, stays in registers.
-    const Request r0 = request(p, min(b0, p.B - 1));
+    Request r0{0, 0, 0};
     auto my_request = [&](int b) { return b == b0 ? r0 : request(p, b); };
-    int64_t my_steps = 0, my_units = 0, total, all_units;
-    for (int b = b0; b < b1; ++b) {
-        const int2 su = steps_and_units<KEYS, ROWS>(p, my_request(b), w.aligned);
-        my_steps += (int64_t)su.x * su.y;
-        my_units += su.y;
+    int64_t steps_before = 0, units_before = 0, total = (int64_t)p.B * units_each;
+    if (!uniform) {
+        r0 = request(p, min(b0, p.B - 1));
+        int64_t my_steps = 0, my_units = 0, all_units;
+        for (int b = b0; b < b1; ++b) {
+            const int2 su = steps_and_units<KEYS, ROWS>(p, my_request(b), w.aligned);
+            my_steps += (int64_t)su.x * su.y;
+            my_units += su.y;
+        }
+        steps_before = prefix_of(my_steps, sh.sum, &total);
+        units_before = prefix_of(my_units, sh.units, &all_units);
     }
-    const int64_t steps_before = prefix_of(my_steps, sh.sum, &total);
-    const int64_t units_before = prefix_of(my_units, sh.units, &all_units);
     const int64_t share = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)w.least);
     const int64_t begin = blockIdx.x * share, end = min(begin + share, total);
     if (p.starts) {  // tokens behind the last request
@@ -230,10 +238,44 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
         return t0 < g.last ? make_int2(t0, min(t0 + per_wave, g.last)) : make_int2(g.first, g.first + 1);
     };
 
+    // Unit u of request b, its steps [x, y) of the line out of [unit_begin, unit_end).
+    auto segment_of = [&](int b, const Request& r, int u, int64_t x, int64_t y, int64_t unit_begin, int64_t unit_end) {
+        Segment g;
+        g.b = b;
+        g.q0 = r.q0;
+        g.n = r.n;
+        g.ctx = r.ctx;
+        g.unit = u;
+        g.row_tile = u / p.Hkv;
+        g.head = u - g.row_tile * p.Hkv;
+        const int rows = min(r.n, p.max_q) * p.G;
+        const int sees = keys_to_scan(p, reach(p, r, (min((g.row_tile + 1) * ROWS, rows) - 1) / p.G));
+        const int turns = (sees + KEYS - 1) / KEYS;
+        g.first = w.aligned ? 0 : (int)(x - unit_begin);
+        g.last = w.aligned ? turns : min((int)(y - unit_begin), turns);
+        g.part = -1;
+        if (x != unit_begin || y != unit_end) {
+            g.part = 2 * blockIdx.x + (x == begin ? 0 : 1);
+            if (x == unit_begin)
+                sh.whole = Whole{r.q0, r.n, r.ctx, g.row_tile, g.head,
+                                 (int)quotient(unit_end - 1, share) - (int)blockIdx.x + 1, g.part, 0};
+        }
+        return g;
+    };
+
     for (int64_t from = begin; from < end;) {
         // The next segments of the share, in order.
+        int count;
         __syncthreads();
-        {
+        if (uniform) {
+            count = (int)min(end - from, (int64_t)kSegments);
+            if (tid < count) {
+                const int64_t at = from + tid;
+                const int b = (int)quotient(at, units_each);
+                sh.list[tid] = segment_of(b, request(p, b), (int)(at - (int64_t)b * units_each), at, at + 1, at, at + 1);
+            }
+            if (tid == 0) sh.behind = from + count;
+        } else {
             int64_t base = steps_before, unit_base = units_before;
             for (int b = b0; b < b1; ++b) {
                 const int2 su = steps_and_units<KEYS, ROWS>(p, my_request(b), w.aligned);
@@ -243,12 +285,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
                 base = after;
                 unit_base += su.y;
             }
-        }
-        __syncthreads();
-        const int64_t unit0 = uniform64(sh.unit0), unit1 = uniform64(sh.unit1);
-        const int count = (int)min(unit1 - unit0 + 1, (int64_t)kSegments);
-        {
-            int64_t base = steps_before, unit_base = units_before;
+            __syncthreads();
+            const int64_t unit0 = uniform64(sh.unit0), unit1 = uniform64(sh.unit1);
+            count = (int)min(unit1 - unit0 + 1, (int64_t)kSegments);
+            base = steps_before;
+            unit_base = units_before;
             for (int b = b0; b < b1; ++b) {
                 const Request r = my_request(b);
                 const int2 su = steps_and_units<KEYS, ROWS>(p, r, w.aligned);
@@ -257,28 +298,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p, Share
                 for (int u = u0; u < u1; ++u) {
                     const int64_t unit_begin = base + (int64_t)u * su.x, unit_end = unit_begin + su.x;
                     const int64_t x = max(from, unit_begin), y = min(end, unit_end);
-                    Segment g;
-                    g.b = b;
-                    g.q0 = r.q0;
-                    g.n = r.n;
-                    g.ctx = r.ctx;
-                    g.unit = u;
-                    g.row_tile = u / p.Hkv;
-                    g.head = u - g.row_tile * p.Hkv;
-                    const int rows = min(r.n, p.max_q) * p.G;
-                    const int sees = keys_to_scan(p, reach(p, r, (min((g.row_tile + 1) * ROWS, rows) - 1) / p.G));
-                    const int turns = (sees + KEYS - 1) / KEYS;
-                    g.first = w.aligned ? 0 : (int)(x - unit_begin);
-                    g.last = w.aligned ? turns : min((int)(y - unit_begin), turns);
-                    g.part = -1;
-                    if (y - x != su.x) {
-                        g.part = 2 * blockIdx.x + (x == begin ? 0 : 1);
-                        if (x == unit_begin)
-                            sh.whole = Whole{r.q0, r.n, r.ctx, g.row_tile, g.head,
-                                             (int)quotient(unit_end - 1, share) - (int)blockIdx.x + 1, g.part, 0};
-                    }
                     const int at = (int)(unit_base + u - unit0);
-                    sh.list[at] = g;
+                    sh.list[at] = segment_of(b, r, u, x, y, unit_begin, unit_end);
                     if (at == count - 1) sh.behind = y;
                 }
                 base += (int64_t)su.x * su.y;
@@ -536,8 +557,13 @@ struct Plan {
 };
 
 // Requests of up to this many rows go to the few-rows kernel, which reads the
-// keys once for each 32 of them and spreads few units over the GPU.
-constexpr int kFewRows = 64;
+// keys once for each 32 of them and spreads them over the GPU.  The prompts'
+// kernel takes 128 rows in about the time of any fewer (e4m3, us, few-rows kernel
+// against prompts'; 32 requests of 500 to 8192 keys, 8 key heads of 128: 64 rows
+// 142 against 279, 128 rows 240 against 303, 192 rows 341 against 311; one of
+// 30000 keys: 128 rows 58 against 65, 192 rows 75 against 67; 16 of 500 to 4096,
+// 2 heads of 256: 128 rows 66 against 73, 192 rows 88 against 75).
+constexpr int kFewRows = 128;
 
 Plan plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int64_t max_ctx) {
     Plan r;

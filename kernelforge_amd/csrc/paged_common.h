@@ -53,20 +53,6 @@ __host__ __device__ __forceinline__ Request request_at(const int* starts, const 
     return r;
 }
 
-// The last request that starts at or before a token, or -1: the one it belongs
-// to, if it belongs to any.
-__host__ __device__ __forceinline__ int request_of(const int* starts, int B, int token) {
-    int lo = 0, hi = B;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= token)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    return lo - 1;
-}
-
 // Keys that query i of a request sees.
 __host__ __device__ __forceinline__ int keys_seen(const Request& r, int i, bool causal) {
     const int seen = causal ? r.ctx - r.n + i + 1 : r.ctx;

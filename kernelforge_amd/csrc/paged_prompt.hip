@@ -10,20 +10,24 @@ constexpr float kPromptPScale = 4096.0f;  // 2^12: a probability may exceed its 
 constexpr float kRise = 3.0f;
 
 // ---------------------------------------------------------------------------
-// Many rows: 64 * RT (query, head) rows of one key head per workgroup, 16 * RT a
-// wavefront, 64 keys at a time through LDS.
+// Many rows: 128 (query, head) rows of one key head per workgroup, 16 for each of
+// eight wavefronts, 64 keys at a time through LDS.
 //
 // The products and their operand layouts are those of the few-rows kernel
 // (paged_attn.hip): S^T = K Q^T leaves each lane the scores of one 16-token
 // group, which are the second product's operand as they are.  Here all
-// wavefronts read the same keys.  Each loads the codes of one of a tile's four
-// groups, whose block, address and scales are scalars, a tile ahead into
-// registers, and writes them into LDS as 16-bit floats behind the first product
+// wavefronts read the same keys.  Two of them load the codes of one of a tile's
+// four groups, whose block, address and scales are scalars, a tile ahead into
+// registers, and write them into LDS as 16-bit floats behind the first product
 // of the tile before; one barrier a tile.
 //
-// Issue-bound (counters: the SIMDs issue in 83% of the cycles, two wavefronts
-// each), so what counts is the instructions for a key: codes that every
-// wavefront converted for itself, behind LDS tiles of codes, ran XX.
+// Issue-bound: of two prompts' chunks of 2048 tokens over 8192 keys, 32 heads of
+// 128 (425 GFLOP, 549 us, 774 TFLOP/s), the SIMDs issue vector instructions in
+// 59% of their cycles and matrix instructions in 36%.  So the instructions for a
+// key count: with the codes in LDS and a conversion by each of four wavefronts of
+// 32 rows it took 592 us.  Four wavefronts of 32 rows over 16-bit tiles take 561
+// (and 138 against 153 at a dim of 64), but are slower on short chunks, which have
+// half as many of them to hide the loads.
 //
 // Keys lie in LDS as rows of 16-byte chunks (8 elements) permuted by key_swizzle,
 // values as [group][column][16 tokens] with the halves of odd groups exchanged;
@@ -83,14 +87,16 @@ template <int ROWS> __device__ __forceinline__ Unit unit_at(const PagedParams& p
     u.r = uniform_request(p, u.b);
     const int row_tile = index - tile_of(u.r.q0, u.b);
     u.row0 = row_tile * ROWS;
-    if ((int64_t)u.r.n * p.G <= p.few || row_tile < 0 || u.row0 >= min(u.r.n, p.max_q) * p.G) u.b = -1;
+    // (in 64 bits: starts that run backwards can lead to any tile)
+    if ((int64_t)u.r.n * p.G <= p.few || row_tile < 0 || (int64_t)row_tile * ROWS >= min(u.r.n, p.max_q) * p.G) u.b = -1;
     return u;
 }
 
 template <typename T, int CT, int DP>
-__global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) void paged_prompt_kernel(PagedParams p, PromptWork w) {
+__global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) void paged_prompt_kernel(
+    PagedParams p, PromptWork w) {
     using Shape = PromptShape<DP>;
-    constexpr int RT = 1, ROWS = Shape::ROWS, CH = Shape::CH, BUFFERS = Shape::BUFFERS;
+    constexpr int ROWS = Shape::ROWS, CH = Shape::CH, BUFFERS = Shape::BUFFERS;
     constexpr int KC = DP / 32, VT = DP / 16;
     constexpr int NC = (DP + 127) / 128;  // 16-byte vectors of half a group's codes a lane
     __shared__ u32x4 s_keys[BUFFERS][64 * CH];
@@ -110,23 +116,19 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
     if (row0 == 0 && blockIdx.y == 0 && r.n > p.max_q)
         fill_rows<T>(p, r.q0 + p.max_q, r.q0 + r.n, 1, head * p.G, p.G, 3, __builtin_nanf(""), __builtin_nanf(""));
 
-    // This wavefront's rows.
-    const int my_row0 = row0 + 16 * RT * wave;
-    int limit[RT];
-    typename V<T>::x8 qf[RT][KC];
+    // This lane's row.
+    const int my_row0 = row0 + 16 * wave;
+    const int row = my_row0 + m, i = row / p.G;
+    const bool live = row < rows;
+    const int limit = live ? reach(p, r, i) : 0;
+    typename V<T>::x8 qf[KC];
+    const T* q = (const T*)p.q + (int64_t)(r.q0 + i) * p.q_ts + (int64_t)(head * p.G + row % p.G) * p.q_hs;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = my_row0 + 16 * rt + m, i = row / p.G;
-        const bool live = row < rows;
-        limit[rt] = live ? reach(p, r, i) : 0;
-        const T* q = (const T*)p.q + (int64_t)(r.q0 + i) * p.q_ts + (int64_t)(head * p.G + row % p.G) * p.q_hs;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int col = 32 * c + 8 * quarter;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (live && col < D) v = *(const u32x4*)(q + col);
-            qf[rt][c] = __builtin_bit_cast(typename V<T>::x8, v);
-        }
+    for (int c = 0; c < KC; ++c) {
+        const int col = 32 * c + 8 * quarter;
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (live && col < D) v = *(const u32x4*)(q + col);
+        qf[c] = __builtin_bit_cast(typename V<T>::x8, v);
     }
     auto seen_by = [&](int row) {
         return __builtin_amdgcn_readfirstlane(keys_to_scan(p, reach(p, r, min(row, rows - 1) / p.G)));
@@ -207,15 +209,10 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
         return s;
     };
 
-    f32x4 acc[RT][VT];
-    float ref[RT], sum[RT], vref = kLeastScale, inv_vref = 1.0f / kLeastScale;
+    f32x4 acc[VT];
+    float ref = -__builtin_inff(), sum = 0.0f, vref = kLeastScale, inv_vref = 1.0f / kLeastScale;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        ref[rt] = -__builtin_inff();
-        sum[rt] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < VT; ++d) acc[rt][d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int d = 0; d < VT; ++d) acc[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     // Operand reads: a lane's chunk of column block c, and its values' halves.
     uint32_t read_k = (16 * (m >> 2) + (m & 3)) * CH + (quarter ^ key_swizzle<CH>(16 * (m >> 2) + (m & 3)));
     const uint32_t read_v = (quarter * DP + m) * 2 + (quarter & 1);
@@ -247,16 +244,14 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
         const float vmax = fmaxf(fmaxf(s_scales[now][0].y, s_scales[now][1].y),
                                  fmaxf(s_scales[now][2].y, s_scales[now][3].y));
         asm volatile("" : "+v"(read_k));  // its columns' addresses are formed here, not kept
-        f32x4 s[RT][4];
+        f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            s[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const auto a = __builtin_bit_cast(typename V<T>::x8, s_keys[now][(read_k ^ (4 * c)) + 4 * t * CH]);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma16x16x32(a, qf[rt][c], s[rt][t]);
+                s[t] = mfma16x16x32(a, qf[c], s[t]);
             }
         }
         if constexpr (BUFFERS == 2) pass_on(now ^ 1);
@@ -264,53 +259,45 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
         const bool edge = 64 * tile + 64 > all_see;
         // The lane's keys share a scale, which is not negative: their largest
         // product is their largest score.
-        float most[RT];
-        bool rise = false;
-        // Keys of this lane's group that a row sees.  The empty asm keeps the
+        float most;
+        // Keys of this lane's group that its row sees.  The empty asm keeps the
         // comparisons out of the tiles that every row sees whole.
-        auto seen_here = [&](int rt) {
-            int n = limit[rt] - key0;
+        auto seen_here = [&] {
+            int n = limit - key0;
             asm volatile("" : "+v"(n));
             return n;
         };
         auto largest = [&](auto at_edge) {
+            if (decltype(at_edge)::value) {
+                const int n = seen_here();
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (decltype(at_edge)::value) {
-                    const int n = seen_here(rt);
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (4 * t + i >= n) s[rt][t][i] = -__builtin_inff();
-                }
-                float x = s[rt][0][0];
-#pragma unroll
-                for (int k = 1; k < 16; ++k) x = fmaxf(x, s[rt][k >> 2][k & 3]);
-                most[rt] = row_max4(x * mine.x);
-                rise |= most[rt] > ref[rt] + kRise;
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * t + i >= n) s[t][i] = -__builtin_inff();
             }
+            float x = s[0][0];
+#pragma unroll
+            for (int k = 1; k < 16; ++k) x = fmaxf(x, s[k >> 2][k & 3]);
+            most = row_max4(x * mine.x);
         };
         if (edge)
             largest(std::true_type());
         else
             largest(std::false_type());
         // The references follow the rows' maxima when one has risen by 2^kRise.
-        if (__any(rise) || vmax > vref) {
+        if (__any(most > ref + kRise) || vmax > vref) {
             const float shrink = vmax > vref ? vref / vmax : 1.0f;
             if (vmax > vref) {
                 vref = vmax;
                 inv_vref = 1.0f / vmax;
             }
+            const float to = fmaxf(ref, most);
+            const float alpha = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+            ref = to;
+            sum *= alpha;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float to = fmaxf(ref[rt], most[rt]);
-                const float alpha = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref[rt] - to);
-                ref[rt] = to;
-                sum[rt] *= alpha;
-#pragma unroll
-                for (int d = 0; d < VT; ++d) acc[rt][d] *= alpha * shrink;
-            }
+            for (int d = 0; d < VT; ++d) acc[d] *= alpha * shrink;
         }
         // exp2(score - reference) * factor as one exponential of one fma; the
         // sum takes the factor out again.  A factor below 2^-60 counts as 2^-60:
@@ -318,25 +305,22 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
         const float factor = mine.y * inv_vref * kPromptPScale;
         const float least = factor < 0x1p-60f ? 0x1p-60f : factor;  // keeps a NaN
         const float lift = __builtin_amdgcn_logf(least), unlift = __builtin_amdgcn_exp2f(-lift);
-        V<f16>::x8 pf[RT][2];
+        V<f16>::x8 pf[2];
         auto probabilities = [&](auto at_edge) {
+            const float base = lift - (ref == -__builtin_inff() ? 0.0f : ref);
+            float add = 0.0f;
+            const int n = decltype(at_edge)::value ? seen_here() : 0;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float base = lift - (ref[rt] == -__builtin_inff() ? 0.0f : ref[rt]);
-                float add = 0.0f;
-                const int n = decltype(at_edge)::value ? seen_here(rt) : 0;
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], mine.x, base));
-                        // A hidden key's weight is 0 whatever its block's scale.
-                        if (decltype(at_edge)::value && 4 * t + i >= n) e = 0.0f;
-                        add += e;
-                        pf[rt][t >> 1][4 * (t & 1) + i] = (f16)e;
-                    }
-                sum[rt] += add == 0.0f ? 0.0f : add * unlift;  // rows that see no key of a NaN scale
-            }
+                for (int i = 0; i < 4; ++i) {
+                    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mine.x, base));
+                    // A hidden key's weight is 0 whatever its block's scale.
+                    if (decltype(at_edge)::value && 4 * t + i >= n) e = 0.0f;
+                    add += e;
+                    pf[t >> 1][4 * (t & 1) + i] = (f16)e;
+                }
+            sum += add == 0.0f ? 0.0f : add * unlift;  // rows that see no key of a NaN scale
         };
         if (edge)
             probabilities(std::true_type());
@@ -347,8 +331,7 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const auto a = __builtin_bit_cast(V<f16>::x8, s_values[now][(read_v ^ h) + 32 * d]);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][d] = mfma16x16x32(a, pf[rt][h], acc[rt][d]);
+                acc[d] = mfma16x16x32(a, pf[h], acc[d]);
             }
         if constexpr (BUFFERS == 1) {
             __syncthreads();
@@ -358,34 +341,30 @@ __global__ __launch_bounds__(64 * PromptShape<DP>::WAVES, PromptShape<DP>::OCC) 
         }
     }
 
+    const float l = row_sum4(sum);
+    if (!live) return;
+    const int token = r.q0 + i, h = head * p.G + row % p.G;
+    if (w.splits > 1) {
+        const int64_t at = ((int64_t)blockIdx.x * w.splits + blockIdx.y) * ROWS + (row - row0);
+        if (quarter == 0) w.to.ml[at] = make_float2(ref, l);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = my_row0 + 16 * rt + m;
-        const float l = row_sum4(sum[rt]);
-        if (row >= rows) continue;
-        const int i = row / p.G, token = r.q0 + i, h = head * p.G + row % p.G;
-        if (w.splits > 1) {
-            const int64_t at = ((int64_t)blockIdx.x * w.splits + blockIdx.y) * ROWS + (row - row0);
-            if (quarter == 0) w.to.ml[at] = make_float2(ref[rt], l);
-#pragma unroll
-            for (int d = 0; d < VT; ++d)
-                if (16 * d < D)
-                    *(f32x4*)(w.to.o + at * D + 16 * d + 4 * quarter) = acc[rt][d] * (1.0f / kPromptPScale) * vref;
-            continue;
-        }
-        const bool none = limit[rt] <= 0;
-#pragma unroll
-        for (int d = 0; d < VT; ++d) {
-            if (16 * d >= D) continue;
-            const f32x4 o = acc[rt][d] * (1.0f / kPromptPScale) * vref;
-            typename V<T>::x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] / l);
-            *(typename V<T>::x4*)((T*)p.out + ((int64_t)token * p.Hq + h) * D + 16 * d + 4 * quarter) = v;
-        }
-        if (p.lse && quarter == 0)
-            p.lse[(int64_t)h * p.tokens + token] = none ? __builtin_inff() : (ref[rt] + log2f(l)) * kLn2;
+        for (int d = 0; d < VT; ++d)
+            if (16 * d < D)
+                *(f32x4*)(w.to.o + at * D + 16 * d + 4 * quarter) = acc[d] * (1.0f / kPromptPScale) * vref;
+        return;
     }
+    const bool none = limit <= 0;
+#pragma unroll
+    for (int d = 0; d < VT; ++d) {
+        if (16 * d >= D) continue;
+        const f32x4 o = acc[d] * (1.0f / kPromptPScale) * vref;
+        typename V<T>::x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.0f : o[e] / l);
+        *(typename V<T>::x4*)((T*)p.out + ((int64_t)token * p.Hq + h) * D + 16 * d + 4 * quarter) = v;
+    }
+    if (p.lse && quarter == 0)
+        p.lse[(int64_t)h * p.tokens + token] = none ? __builtin_inff() : (ref + log2f(l)) * kLn2;
 }
 
 // Joins a unit's splits, in order: LANES threads with eight columns each a row.

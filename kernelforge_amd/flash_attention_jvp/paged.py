@@ -83,20 +83,24 @@ def _check_layout(head_dim, block_tokens, dtype):
 def _check_cache(cache, device):
     """(blocks, Hkv, T, D) of a cache whose tensors all fit one another."""
     key, value, key_scale, value_scale = cache
-    if key.ndim != 4 or min(key.shape) < 1:
+    shape = key.shape
+    if len(shape) != 4 or 0 in shape:
         raise ValueError("the key cache must have shape [blocks, heads, block_tokens, dim]")
-    blocks, heads, T, D = key.shape
-    _check_layout(D, T, key.dtype)
-    if value.shape != (blocks, heads, T // 16, D, 16) or value.dtype != key.dtype:
+    blocks, heads, T, D = shape
+    dtype = key.dtype
+    _check_layout(D, T, dtype)
+    if value.shape != (blocks, heads, T // 16, D, 16) or value.dtype != dtype:
         raise ValueError("the value cache must have shape [blocks, heads, block_tokens / 16, dim, 16] and the keys' dtype")
-    for scale in (key_scale, value_scale):
-        if scale.shape != (blocks, heads) or scale.dtype != torch.float32:
-            raise ValueError("the cache's scales must be float32 [blocks, heads]")
-    for t in (key, value, key_scale, value_scale):
-        if not t.is_contiguous():
-            raise ValueError("the cache's tensors must be contiguous")
-        if t.device != device:
-            raise ValueError("the cache must be on the call's device")
+    pair = (blocks, heads)
+    f32 = torch.float32
+    if (key_scale.shape != pair or key_scale.dtype != f32 or value_scale.shape != pair or value_scale.dtype != f32):
+        raise ValueError("the cache's scales must be float32 [blocks, heads]")
+    if not (key.is_contiguous() and value.is_contiguous() and key_scale.is_contiguous()
+            and value_scale.is_contiguous()):
+        raise ValueError("the cache's tensors must be contiguous")
+    if (key.device != device or value.device != device or key_scale.device != device
+            or value_scale.device != device):
+        raise ValueError("the cache must be on the call's device")
     return blocks, heads, T, D
 
 
@@ -109,17 +113,21 @@ def _check_ints(name, t, shape, dtype, device):
 
 
 def _check_no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("the paged operators have no backward: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("the paged operators have no backward: call them under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [tokens, heads, D] itself where its rows can be read as 16-byte vectors (a
-    part of a packed projection can), else a copy."""
+def _rows(t: torch.Tensor):
+    """t [tokens, heads, D] and its strides of tokens and heads, where its rows can
+    be read as 16-byte vectors (a part of a packed projection can), else a copy's."""
     st, sh, sd = t.stride()
-    if sd == 1 and st % 8 == 0 and 0 <= st < 1 << 26 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    if sd == 1 and st % 8 == 0 and st < 1 << 26 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, st, sh
+    # (a contiguous tensor's clone keeps the strides of its dimensions of one)
+    t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t, *t.stride()[:2]
 
 
 def _on(index: int):
@@ -166,10 +174,12 @@ def paged_block_tables_(block_tables, context_lens, query_lens, free_blocks, fre
     _check_ints("free_blocks", free_blocks, free_blocks.shape, i32, device)
     _check_ints("free_used", free_used, (1,), i32, device)
     _lib.require_gpu(block_tables)
-    starts = torch.empty(B + 1, dtype=i32, device=device)
-    slots = torch.empty(total_tokens, dtype=torch.int64, device=device)
-    context, used = (context_lens, free_used) if in_place else (torch.empty_like(context_lens),
-                                                               torch.empty_like(free_used))
+    empty = torch.empty
+    starts = empty(B + 1, dtype=i32, device=device)
+    slots = empty(total_tokens, dtype=torch.int64, device=device)
+    context, used = context_lens, free_used
+    if not in_place:
+        context, used = empty(B, dtype=i32, device=device), empty(1, dtype=i32, device=device)
     with _on(device.index):
         rc = _lib.load().kf_paged_block_tables(
             block_tables.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(), free_blocks.data_ptr(),
@@ -210,18 +220,19 @@ def paged_cache_append_(cache, key, value, slots):
     _check_no_grad(key, value)
     if tokens == 0:
         return cache
-    key, value = _rows(key), _rows(value)
+    (key, key_ts, key_hs), (value, value_ts, value_hs) = _rows(key), _rows(value)
+    kc, vc, ks, vs = cache
     with _on(device.index):
         rc = _lib.load().kf_paged_cache_append(
-            key.data_ptr(), value.data_ptr(), slots.data_ptr(), *(t.data_ptr() for t in cache), tokens, blocks, heads,
-            D, T, key.stride(0), key.stride(1), value.stride(0), value.stride(1), _lib.kf_dtype(key.dtype),
-            _CACHE_DTYPES[cache[0].dtype], _lib.stream_of(key))
+            key.data_ptr(), value.data_ptr(), slots.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(),
+            vs.data_ptr(), tokens, blocks, heads, D, T, key_ts, key_hs, value_ts, value_hs, _lib.kf_dtype(key.dtype),
+            _CACHE_DTYPES[kc.dtype], _lib.stream_of(key))
     _lib.check(rc, "kf_paged_cache_append")
     return cache
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(device: torch.device, *shape) -> int:
+def _workspace_bytes(device_index: int, *shape) -> int:
     """``kf_paged_attention_workspace_bytes`` of a shape on a device (the current one)."""
     return int(_lib.load().kf_paged_attention_workspace_bytes(*shape))
 
@@ -255,16 +266,18 @@ def paged_attention(q, cache, block_tables, context_lens, query_starts=None, *, 
         raise ValueError("q must be float16 or bfloat16 of shape [tokens, heads, dim]")
     device = q.device
     blocks, Hkv, T, D = _check_cache(cache, device)
-    tokens, Hq = q.shape[:2]
-    if q.shape[2] != D or Hq < 1 or Hq % Hkv:
+    tokens, Hq, dim = q.shape
+    if dim != D or Hq < 1 or Hq % Hkv:
         raise ValueError("q must have the cache's head dim and a multiple of its heads")
-    if block_tables.ndim != 2 or min(block_tables.shape) < 1:
+    table_shape = block_tables.shape
+    if len(table_shape) != 2 or 0 in table_shape:
         raise ValueError("block_tables must be int32 [requests, width], neither of them 0")
-    B, width = block_tables.shape
-    _check_ints("block_tables", block_tables, (B, width), torch.int32, device)
-    _check_ints("context_lens", context_lens, (B,), torch.int32, device)
+    B, width = table_shape
+    i32 = torch.int32
+    _check_ints("block_tables", block_tables, table_shape, i32, device)
+    _check_ints("context_lens", context_lens, (B,), i32, device)
     if query_starts is not None:
-        _check_ints("query_starts", query_starts, (B + 1,), torch.int32, device)
+        _check_ints("query_starts", query_starts, (B + 1,), i32, device)
     elif tokens != B:
         raise ValueError("without query_starts q must hold one token of every request")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
@@ -287,22 +300,27 @@ def paged_attention(q, cache, block_tables, context_lens, query_starts=None, *, 
     _check_no_grad(q)
     given = out is not None
     if not given:
-        out = torch.empty((tokens, Hq, D), dtype=q.dtype, device=device)
+        out = torch.empty(tokens, Hq, D, dtype=q.dtype, device=device)
     lse = torch.empty((Hq, tokens), dtype=torch.float32, device=device) if return_lse else None
     if tokens == 0:
         return (out, lse) if return_lse else out
-    q = _rows(q)
-    shape = (tokens, B, Hq, Hkv, D, min(max_query_len, tokens), min(max_context_len, width * T))
-    with _on(device.index):
-        nbytes = _workspace_bytes(device, *shape)
+    q, q_ts, q_hs = _rows(q)
+    kc, vc, ks, vs = cache
+    if max_query_len > tokens:
+        max_query_len = tokens
+    if max_context_len > width * T:
+        max_context_len = width * T
+    index = device.index
+    with _on(index):
+        nbytes = _workspace_bytes(index, tokens, B, Hq, Hkv, D, max_query_len, max_context_len)
         if nbytes < 0:
             raise ValueError(f"paged_attention: {_lib.load().kf_last_error().decode()}")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = _lib.load().kf_paged_attention(
-            q.data_ptr(), *(t.data_ptr() for t in cache), block_tables.data_ptr(), context_lens.data_ptr(),
-            None if query_starts is None else query_starts.data_ptr(), out.data_ptr(),
+            q.data_ptr(), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), block_tables.data_ptr(),
+            context_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), out.data_ptr(),
             None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, tokens, B, blocks,
-            width, Hq, Hkv, D, T, q.stride(0), q.stride(1), shape[5], shape[6], scale, bool(causal), 2 if given else 3,
-            _lib.kf_dtype(q.dtype), _CACHE_DTYPES[cache[0].dtype], _lib.stream_of(q))
+            width, Hq, Hkv, D, T, q_ts, q_hs, max_query_len, max_context_len, scale, bool(causal), 2 if given else 3,
+            _lib.kf_dtype(q.dtype), _CACHE_DTYPES[kc.dtype], _lib.stream_of(q))
     _lib.check(rc, "kf_paged_attention")
     return (out, lse) if return_lse else out

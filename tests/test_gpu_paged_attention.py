@@ -330,6 +330,133 @@ def test_against_flash_attention():
         torch.testing.assert_close(mine.float(), dense.float(), rtol=2.0 ** -7, atol=2.0 ** -7 * 2)
 
 
+@pytest.mark.parametrize("code,dtype", [(E4M3, torch.float16), (INT8, torch.bfloat16)])
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(16, 8, 2, 128), (64, 4, 4, 64), (32, 8, 1, 256), (128, 6, 2, 96), (16, 3, 1, 16)])
+def test_rows_around_the_kernels_border(T, Hq, Hkv, D, code, dtype):
+    """Requests of just up to 128 rows of a key head and just past them, in one call
+    and alone, cut and whole."""
+    rng = random.Random(D + 1)
+    group = Hq // Hkv
+    count = [128 // group, 128 // group + 1, 1, 128 // group - 1]
+    context = [900, 1100, 1500, 90]
+    starts = [0]
+    for n in count:
+        starts.append(starts[-1] + n)
+    cache = make_cache(260, Hkv, T, D, code)
+    tables = layout(context, T, 260, rng)
+    q = queries(starts[-1], Hq, D, dtype)
+    check(q, cache, tables, context, starts, max_query_len=max(count))
+    check(q, cache, tables, context, starts, max_query_len=max(count), max_context_len=0)
+    for b in (0, 1):
+        check(q[starts[b]:starts[b + 1]], cache, tables[b:b + 1], context[b:b + 1], [0, count[b]], causal=False)
+
+
+@pytest.mark.parametrize("bad", [-1, 90, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("n,context", [(100, 170), (300, 1100)])
+def test_bad_pages_of_a_prompt(n, context, bad):
+    """Many rows over a missing block, with one workgroup a unit and with several."""
+    T, D, at = 16, 64, 5
+    rng = random.Random(7)
+    cache = make_cache(90, 2, T, D, E4M3)
+    tables = layout([context], T, 90, rng)
+    tables[0][(context - n) // T + at] = bad
+    q = queries(n, 8, D, torch.bfloat16)
+    first = ((context - n) // T + at) * T - (context - n)  # the first query that sees the block
+    out, lse = check(q, cache, tables, [context], [0, n])
+    assert out[:first].isfinite().all() and out[first:].isnan().all()
+    out = paged_attention(q, cache, ints([tables[0][:(context - n) // T + at]]), ints([context]), ints([0, n]))
+    assert out[:first].isfinite().all() and out[first:].isnan().all()
+
+
+@pytest.mark.parametrize("T,n,context", [(16, 100, 170), (64, 300, 1111)])
+def test_poison_in_a_prompt(T, n, context):
+    """Scales and codes that only some rows see, and what lies behind the context."""
+    D, blocks = 64, 90
+    rng = random.Random(8)
+    cache = make_cache(blocks, 2, T, D, E4M3)
+    tables = layout([context], T, blocks, rng, width=-(-context // T) + 3)
+    q = queries(n, 8, D, torch.bfloat16)
+    want = check(q, cache, tables, [context], [0, n])
+    at = (context - n) // T + 1
+    first = at * T - (context - n)
+    for which, poison in ((2, math.nan), (3, math.nan), (3, math.inf)):
+        parts = [t.clone() for t in cache]
+        parts[which][tables[0][at], 1] = poison
+        out = paged_attention(q, parts, ints(tables), ints([context]), ints([0, n]))
+        assert out[:first].isfinite().all() and torch.equal(out[:, :4], want[0][:, :4])
+        assert out[first:, 4:].isnan().all()
+    raw = [t.view(torch.uint8) for t in cache[:2]]
+    row, rest = tables[0], context % T
+    raw[0][row[context // T], :, rest:] = 0x7f
+    for token in range(rest, T):
+        raw[1][row[context // T], :, token // 16, :, token % 16] = 0xff
+    used = {i for i in row if i >= 0}
+    spare = min(set(range(blocks)) - used)
+    cache.key_scale[spare], cache.value_scale[spare] = math.nan, math.inf
+    row[-3:] = [spare, 2 ** 31 - 1, -2 ** 31]
+    for have, expect in zip(paged_attention(q, cache, ints(tables), ints([context]), ints([0, n]), return_lse=True), want):
+        assert torch.equal(have, expect)
+
+
+def test_lengths_that_lie_in_prompts():
+    """As in the few-rows kernel: NaN or nothing, and nothing outside the tensors."""
+    T, D = 16, 64
+    cache = make_cache(12, 2, T, D, E4M3)
+    tables = ints([[0, 1, 2], [3, 4, 5], [6, 7, 8]])
+    q = queries(400, 4, D, torch.float16)
+    starts = ints([0, 150, 300, 400])
+    out = paged_attention(q, cache, tables, ints([2 ** 31 - 1, 48, -2 ** 31]), starts)
+    assert out[:150].isnan().all() and out[150:300].isfinite().all() and not out[300:].any()
+    out = paged_attention(q, cache, tables, ints([40, 40, 40]), starts, max_query_len=120)
+    want = paged_attention(q, cache, tables, ints([40, 40, 40]), starts)
+    for b, n in ((0, 150), (150, 150), (300, 100)):
+        assert torch.equal(out[b:b + min(n, 120)], want[b:b + min(n, 120)]) and out[b + 120:b + n].isnan().all()
+    for lie in ([0, 300, 0, 300], [399, 2, 2 ** 31 - 1, 7], [-2 ** 31, 2 ** 31 - 1, -1, 400], [400, 0, 400, 0]):
+        paged_attention(q, cache, tables, ints([40, 40, 40]), ints(lie))
+    torch.cuda.synchronize()
+
+
+def test_prompts_on_another_stream_and_captured():
+    """A batch that takes both kernels and both joins, in two graphs that are
+    replayed in turn on changed inputs, with eager work between."""
+    T, D = 16, 128
+    cache = make_cache(600, 2, T, D, INT8)
+    tables, context, starts = ints([list(range(300)), list(range(300, 600))]), ints([4000, 4500]), ints([0, 1, 201])
+    args = (cache, tables, context, starts)
+    inputs = [queries(201, 8, D, torch.bfloat16, seed=k) for k in range(3)]
+    want = [paged_attention(x, *args) for x in inputs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = paged_attention(inputs[0], *args)
+    here = paged_attention(inputs[1], *args)  # at the same time
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want[0]) and torch.equal(here, want[1])
+    static, graphs, outs = [inputs[0].clone(), inputs[1].clone()], [], []
+    for x in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention(x, *args))
+        graphs.append(graph)
+    for k in (0, 2, 1, 2):
+        static[0].copy_(inputs[k])
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[k]) and torch.equal(outs[1], want[1])
+        assert torch.equal(paged_attention(inputs[2], *args), want[2])
+
+
+def test_one_head_of_any_stride():
+    """A dimension of one may have any stride (a view of [tokens, D])."""
+    cache = make_cache(4, 1, 16, 64, INT8)
+    tables, context = ints([[0, 1], [2, 3]]), ints([20, 32])
+    q = queries(2, 1, 64, torch.bfloat16)
+    want = paged_attention(q, cache, tables, context)
+    assert torch.equal(paged_attention(q.as_strided((2, 1, 64), (64, 1, 1)), cache, tables, context), want)
+    assert torch.equal(paged_attention(q[:1].as_strided((1, 1, 64), (3, 5, 1)), cache, tables[:1], context[:1]), want[:1])
+
+
 def test_past_32_bits():
     """Blocks whose bytes lie past 2^32 in the caches."""
     T, H, D = 128, 8, 128
