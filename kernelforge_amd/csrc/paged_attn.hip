@@ -573,9 +573,13 @@ Plan plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t
     if (r.prompts) rows = kFewRows;
     r.rt = rows <= 16 || D > 128 ? 1 : 2;
     const int64_t units = B * ((rows + 16 * r.rt - 1) / (16 * r.rt)) * Hkv;
-    // A second launch joins the parts of cut units (5 us).  One workgroup takes
-    // 1024 keys in about as much.
-    r.aligned = max_ctx <= 1024;
+    // A second launch joins the parts of cut units (5 us).  Whole units take less
+    // where the contexts are short (us, whole against cut): of one tile of rows and
+    // a dim of 128, one request of 2000 keys 17.6 against 18.2, of 4000 27 against
+    // 18, 64 of 2000 52 against 56, 128 of 500 to 4000 153 against 122; with two
+    // tiles or a dim of 256 a turn takes longer: one request of 1000 keys 20.4
+    // against 18.4, of 750 17.9 against 17.9, 16 of 1000 21 against 25.
+    r.aligned = max_ctx <= (r.rt == 1 && D <= 128 ? 2048 : 1024);
     // One workgroup a CU streams fastest (two requests of 100000 keys, 16 units: 82
     // us against 86 with two, which fit); a second hides the ends of the first's
     // units where each workgroup may have several (32 requests of 500 to 8192 keys,
@@ -623,10 +627,13 @@ int check_shape(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
     KF_REQUIRE(Hq % Hkv == 0, KF_E_INVALID, "kf_paged_attention: Hq must be a multiple of Hkv");
     KF_REQUIRE(D >= 16 && D <= 256 && D % 16 == 0, KF_E_INVALID,
                "kf_paged_attention: head dim must be a multiple of 16 <= 256");
-    KF_REQUIRE(tokens <= INT32_MAX / 2 && Hq <= INT32_MAX / 2 && B <= INT32_MAX / 2 && tokens * Hq <= INT32_MAX / 2 &&
-                   (tokens * (Hq / Hkv) / 64 + B) * Hkv <= INT32_MAX / 2 && Hkv <= 65535 &&
-                   max_q * (Hq / Hkv) <= INT32_MAX / 2 && B * ((max_q * (Hq / Hkv) + 15) / 16) <= INT32_MAX / 2,
+    KF_REQUIRE(tokens <= INT32_MAX / 2 && Hq <= INT32_MAX / 2 && B <= INT32_MAX / 2 && max_q <= INT32_MAX / 2 &&
+                   tokens * Hq <= INT32_MAX / 2 && Hkv <= 65535 && max_q * (Hq / Hkv) <= INT32_MAX / 2,
                KF_E_UNSUPPORTED, "kf_paged_attention: too many rows");
+    // The prompts' kernel has a workgroup for each of its units, and a launch holds
+    // less than 2^32 threads.
+    KF_REQUIRE(max_q * (Hq / Hkv) <= kFewRows || prompt_plan(tokens, B, Hq, Hkv, D, max_ctx).units < 1 << 23,
+               KF_E_UNSUPPORTED, "kf_paged_attention: too many requests of many rows");
     return KF_OK;
 }
 

@@ -154,11 +154,12 @@ __global__ __launch_bounds__(kTableThreads) void paged_tables_kernel(TableParams
 // ---------------------------------------------------------------------------
 // Writes into the cache.
 //
-// One workgroup handles a run: consecutive tokens of the call whose slots lie
-// in one block.  A unit is the block's keys or values of one head, and each of
-// its 16-token groups has a wavefront, so a unit's elements stay in registers
-// between the maximum that sets the scale and the rounding: the call reads its
-// inputs once and writes the codes once.
+// One workgroup handles the runs that begin in its slice of the tokens, one after
+// the other: consecutive tokens of the call whose slots lie in one block, found by
+// ballots over the slots of 64 tokens.  A unit is the block's keys or values of
+// one head, and each of its 16-token groups has a wavefront, so a unit's elements
+// stay in registers between the maximum that sets the scale and the rounding: the
+// call reads its inputs once and writes the codes once.
 //
 // The scale is the least power of two s >= 2^-126 with max|x| <= M s (M the
 // largest code, 448 or 127) and never shrinks while the block fills.  x / s is
@@ -572,8 +573,9 @@ int kf_paged_cache_append(const void* key, const void* value, const int64_t* slo
     KF_REQUIRE(dtype == KF_F16 || dtype == KF_BF16, KF_E_INVALID, "kf_paged_cache_append: dtype must be f16 or bf16");
     KF_REQUIRE(cache_dtype == KF_CACHE_E4M3 || cache_dtype == KF_CACHE_INT8, KF_E_INVALID,
                "kf_paged_cache_append: bad cache dtype");
-    KF_REQUIRE(blocks <= INT32_MAX && Hkv <= 16384 && tokens <= INT32_MAX, KF_E_UNSUPPORTED,
-               "kf_paged_cache_append: at most 2^31-1 blocks and tokens and 16384 heads");
+    // (a launch holds less than 2^32 threads)
+    KF_REQUIRE(blocks <= INT32_MAX && Hkv <= 16384 && tokens < 1 << 27, KF_E_UNSUPPORTED,
+               "kf_paged_cache_append: at most 2^31-1 blocks, 2^27-1 tokens and 16384 heads");
     if (tokens == 0) return KF_OK;
     KF_REQUIRE(key && value && slots && key_cache && value_cache && key_scale && value_scale, KF_E_INVALID,
                "kf_paged_cache_append: null pointer");
@@ -595,11 +597,20 @@ int kf_paged_cache_append(const void* key, const void* value, const int64_t* slo
                    (int)D,
                    shift,
                    1};
-    const int groups = 1 << (shift - 4), waves = groups > 4 ? groups : 4;
+    const int bt = 1 << shift, groups = bt >> 4, waves = groups > 4 ? groups : 4;
     const int64_t gy = (2 * Hkv * groups + waves - 1) / waves;
-    // Decoding gives every token a block of its own: a workgroup each.  Prompts
-    // begin a run every block_tokens tokens: a workgroup for 16.
-    p.slice = tokens * gy <= 4096 ? 1 : 16;
+    // Tokens of a workgroup.  Decoding gives every token a block of its own, so one
+    // each spreads the runs; prompts begin a run every block_tokens tokens, and most
+    // workgroups of one token find nothing.  The host cannot tell the two apart, so
+    // 2048 workgroups, eight a CU, decide (8 heads of 128, T = 16, us with 1, 2, 4,
+    // 8, 16 tokens each; calls below 9 us wait for the host): 256 requests 10, 10,
+    // 14, 25, 45; 1024 requests 25, 23, 23, 30, 49; 4096 requests 82, 71, 67, 68, 75;
+    // four prompts of 256 tokens 11, 10, 11, 8, 9; of 1000 28, 17, 15, 11, 11.  At
+    // most a block, and the 64 slots that a wavefront looks at (T = 64, 16 against
+    // 64 tokens: two prompts of 4000 40, 18; 2048 requests 136, 152).
+    const int most = bt < 64 ? bt : 64;
+    p.slice = 1;
+    while (p.slice < most && p.slice * 2048 < tokens * gy) p.slice *= 2;
     const int64_t gx = (tokens + p.slice - 1) / p.slice;
     const dim3 grid((unsigned)gx, (unsigned)gy);
     const hipStream_t s = (hipStream_t)stream;

@@ -47,7 +47,7 @@ class PagedKVCache(NamedTuple):
 
     key ``[blocks, Hkv, T, D]`` and value ``[blocks, Hkv, T/16, D, 16]`` (the 16
     tokens of a group innermost) in e4m3 or int8, T the block's tokens; fp32
-    scales ``[blocks, Hkv]``.  An element is its code times its scale.
+    scales ``[blocks, Hkv]``, none negative.  An element is its code times its scale.
     """
 
     key: torch.Tensor
@@ -259,7 +259,7 @@ def paged_attention(q, cache, block_tables, context_lens, query_starts=None, *, 
     max_query_len bounds the new tokens of a request (default: all of q's) and
     has to hold: the queries of a request past it give NaN.  max_context_len
     (default: the table's width) only guides how the keys are split over
-    workgroups.  Results do not depend on the rest of the batch beyond the last
+    workgroups.  out may be q itself, and overlap nothing else.  Results do not depend on the rest of the batch beyond the last
     place, and are the same at every repeat.  There is no backward.
     """
     if q.ndim != 3 or q.dtype not in (torch.float16, torch.bfloat16):
@@ -297,9 +297,11 @@ def paged_attention(q, cache, block_tables, context_lens, query_starts=None, *, 
                             or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be contiguous and have q's shape, dtype, and device")
     _lib.require_gpu(q)
-    _check_no_grad(q)
     given = out is not None
-    if not given:
+    if given:
+        _check_no_grad(q, out)
+    else:
+        _check_no_grad(q)
         out = torch.empty(tokens, Hq, D, dtype=q.dtype, device=device)
     lse = torch.empty((Hq, tokens), dtype=torch.float32, device=device) if return_lse else None
     if tokens == 0:

@@ -351,6 +351,53 @@ def test_rows_around_the_kernels_border(T, Hq, Hkv, D, code, dtype):
         check(q[starts[b]:starts[b + 1]], cache, tables[b:b + 1], context[b:b + 1], [0, count[b]], causal=False)
 
 
+@pytest.mark.parametrize("B,Hkv", [(700, 2), (4200, 8)])
+def test_large_batches(B, Hkv):
+    """Several requests for each thread of the sums, more units than a workgroup
+    lists at a time, a search over many requests: the requests of a call of their
+    own, whole and cut, with and without starts, some of them empty or prompts."""
+    T, D = 16, 16
+    rng = random.Random(B)
+    cache = make_cache(64, Hkv, T, D, INT8, spread=0.0)
+    context = [rng.choice([0, 1, 16, 17, 40]) for _ in range(B)]
+    table = ints([[rng.randrange(64) for _ in range(3)] for _ in range(B)])
+    q = queries(B, 2 * Hkv, D, torch.float16)
+    some = sorted(rng.sample(range(B), 40)) + [B - 1]
+    got = paged_attention(q, cache, table, ints(context), return_lse=True)
+    for kw in (dict(), dict(query_starts=ints(range(B + 1)), max_query_len=1)):
+        for bound in (0, 10 ** 6):
+            same = paged_attention(q, cache, table, ints(context), return_lse=True, max_context_len=bound, **kw)
+            assert torch.equal(same[0], got[0]) and torch.equal(same[1], got[1])
+    want = orc.attention(q[some], cache, table[some].tolist(), [context[b] for b in some], None)
+    compare((got[0][some], got[1][:, some]), want, bounds(want, q.dtype, cache, D, 40))
+    # Of several tokens each, a few of them many; the ones looked at are called alone.
+    count = [rng.choice([0, 1, 1, 2, 3]) for _ in range(B)]
+    for b in rng.sample(range(B), 9):
+        count[b] = rng.randrange(60, 200)
+    starts = [0]
+    for n in count:
+        starts.append(starts[-1] + n)
+    q = queries(starts[-1], 2 * Hkv, D, torch.float16)
+    long = [b for b in range(B) if count[b] > 3]
+    both = [paged_attention(q, cache, table, ints(context), ints(starts), return_lse=True, max_query_len=200,
+                            max_context_len=bound) for bound in (0, 10 ** 6)]
+    for b in long + some:
+        at = slice(starts[b], starts[b + 1])
+        want = orc.attention(q[at], cache, table[b:b + 1].tolist(), context[b:b + 1], [0, count[b]])
+        for out, lse in both:
+            compare((out[at], lse[:, at]), want, bounds(want, q.dtype, cache, D, 40))
+
+
+def test_out_may_be_the_queries():
+    T, D = 16, 64
+    cache = make_cache(200, 2, T, D, INT8)
+    context, starts = ints([3000, 60, 80]), ints([0, 1, 2, 152])
+    tables = ints([list(range(190)), [190] * 190, [191 + k % 9 for k in range(190)]])
+    q = queries(152, 8, D, torch.bfloat16)
+    want = paged_attention(q, cache, tables, context, starts)
+    assert torch.equal(paged_attention(q, cache, tables, context, starts, out=q), want)
+
+
 @pytest.mark.parametrize("bad", [-1, 90, 2 ** 31 - 1, -2 ** 31])
 @pytest.mark.parametrize("n,context", [(100, 170), (300, 1100)])
 def test_bad_pages_of_a_prompt(n, context, bad):

@@ -155,6 +155,31 @@ def test_append_many_runs_in_a_slice(code):
     check_append(cache, key, value, slots)
 
 
+@pytest.mark.parametrize("T,heads,count", [(16, 32, 150), (32, 8, 300), (32, 32, 700), (64, 8, 300), (64, 32, 500),
+                                           (64, 32, 1400), (128, 32, 1400), (128, 32, 2500)])
+def test_append_slices_of_every_length(T, heads, count):
+    """Workgroups of 2 to 64 tokens: prompts whose runs end anywhere in a slice,
+    decoding tokens between them, runs around the 64th slot, padding at the end."""
+    D, blocks = 16, 300
+    rng = random.Random(count + T)
+    cache = filled(blocks, heads, T, D, INT8 if count % 200 else E4M3)
+    slots, order = [], rng.sample(range(blocks), blocks)
+    while len(slots) < count:
+        if rng.random() < 0.6:  # a prompt behind some cached tokens
+            at, n = rng.randrange(T), rng.randrange(1, 3 * T)
+            while n > 0:
+                block, here = order.pop(), min(n, T - at)
+                slots += [block * T + at + i for i in range(here)]
+                at, n = 0, n - here
+        else:
+            slots += [order.pop() * T + rng.randrange(T) for _ in range(rng.randrange(1, 6))]
+        if rng.random() < 0.2:
+            slots += [-1] * rng.randrange(1, 70)
+    slots += [-1] * 3
+    key, value = tokens(len(slots), heads, D, torch.float16)
+    check_append(cache, key, value, slots)
+
+
 @pytest.mark.parametrize("code", [E4M3, INT8])
 def test_append_the_same_slot_twice(code):
     """Of two tokens of a run that name one slot the later is kept, alone."""
