@@ -3,7 +3,8 @@
  *
  * Plain C entry points for the three operator hot paths of KernelForge
  * (RMSNorm, SANA ReLU linear attention with its rotary embedding,
- * FlashAttention forward / JVP / backward), implemented as hand-written HIP
+ * FlashAttention forward / JVP / backward), and for a paged 8-bit key/value
+ * cache with the attention that reads it, implemented as hand-written HIP
  * kernels for gfx950 (MI355X).
  *
  * Conventions shared by every entry point:
@@ -11,7 +12,8 @@
  *     allocates device memory; SANA's cross-split partials and the FA
  *     backward's per-row statistics live in caller-supplied workspaces whose
  *     sizes are given by kf_linattn_workspace_bytes and
- *     kf_fa_bwd_workspace_bytes.
+ *     kf_fa_bwd_workspace_bytes; likewise the paged attention's parts of
+ *     split units (kf_paged_attention_workspace_bytes).
  *   - Tensors are dense and row-major (the innermost dimension is contiguous)
  *     in the layouts documented per function.
  *   - `stream` is a hipStream_t (NULL = the default stream).  Launches are
@@ -544,7 +546,8 @@ int kf_paged_block_tables(int32_t* block_tables, const int32_t* context_lens, co
  *
  * key, value: [tokens, Hkv, D] of `dtype` (f16 or bf16) with the given strides
  * in elements (multiples of 8, those of tokens below 2^26; the dim is
- * contiguous, 16-byte aligned).  Slots outside the cache are skipped.
+ * contiguous, 16-byte aligned); tokens below 2^27.  Slots outside the cache are
+ * skipped.
  * The tokens of one block must follow one another in the call, as the tokens
  * of one request do (of two that name one slot the later is kept); else the
  * codes of that block are unspecified.
@@ -569,11 +572,13 @@ int64_t kf_paged_attention_workspace_bytes(int64_t tokens, int64_t B, int64_t Hq
  *   out = sum_j exp(s_j - lse) * value_scale * value code_j.
  * A row that sees no key gives out = 0 and lse = +inf.  A row that sees a key
  * of a table entry outside the cache, or a key past the table's width, gives
- * NaN.  Codes must be finite where they are read (kf_paged_cache_append writes
- * no others); what lies behind a request's context is not looked at.
+ * NaN.  Codes must be finite where they are read and scales not negative
+ * (kf_paged_cache_append writes no others); what lies behind a request's context
+ * is not looked at.
  *
  * q: [tokens, Hq, D] of dtype (f16 or bf16), strides in elements (multiples of
- * 8), 16-byte aligned rows; out: [tokens, Hq, D] contiguous; lse: [Hq, tokens]
+ * 8), 16-byte aligned rows; out: [tokens, Hq, D] contiguous (q itself, where
+ * that is contiguous, or apart from it); lse: [Hq, tokens]
  * or NULL.  Rows of tokens behind the last request are left as they are,
  * except that clear_rest & 1 writes 0 into out and clear_rest & 2 +inf into
  * lse there.  Queries of a request past max_query_len give NaN.

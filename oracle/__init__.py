@@ -18,4 +18,8 @@ How each function is pinned (beyond restating the reference):
   value-only tangents -> tO = P tV, probability-mass preservation, and the
   tiled online recurrence (``fa.fused_forward_jvp_tiled``) against the dense
   jvp at several tile sizes.
+- ``paged`` (no counterpart in the reference): tables and slots against a
+  case worked by hand, scales and codes against their definition (the least
+  power of two that fits, the nearest code, ties to even), attention against
+  ``fa`` on the elements that the cache stands for.
 """
