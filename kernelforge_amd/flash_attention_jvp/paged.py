@@ -174,12 +174,11 @@ def paged_block_tables_(block_tables, context_lens, query_lens, free_blocks, fre
     _check_ints("free_blocks", free_blocks, free_blocks.shape, i32, device)
     _check_ints("free_used", free_used, (1,), i32, device)
     _lib.require_gpu(block_tables)
-    empty = torch.empty
-    starts = empty(B + 1, dtype=i32, device=device)
-    slots = empty(total_tokens, dtype=torch.int64, device=device)
-    context, used = context_lens, free_used
-    if not in_place:
-        context, used = empty(B, dtype=i32, device=device), empty(1, dtype=i32, device=device)
+    slots = torch.empty(total_tokens, dtype=torch.int64, device=device)
+    if in_place:
+        starts, context, used = torch.empty(B + 1, dtype=i32, device=device), context_lens, free_used
+    else:  # parts of one allocation (an allocation takes the host 1.2 us, as the split does)
+        starts, context, used = torch.empty(2 * B + 2, dtype=i32, device=device).split_with_sizes((B + 1, B, 1))
     with _on(device.index):
         rc = _lib.load().kf_paged_block_tables(
             block_tables.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(), free_blocks.data_ptr(),
