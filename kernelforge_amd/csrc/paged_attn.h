@@ -52,6 +52,7 @@ struct PromptPlan {
     int splits;
     int64_t bytes;
 };
+int64_t prompt_units(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv);
 PromptPlan prompt_plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_ctx);
 int launch_prompt(const PagedParams& p, const PromptPlan& w, void* workspace, int dtype, int cache_dtype,
                   hipStream_t stream);

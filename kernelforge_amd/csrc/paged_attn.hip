@@ -632,7 +632,7 @@ int check_shape(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
                KF_E_UNSUPPORTED, "kf_paged_attention: too many rows");
     // The prompts' kernel has a workgroup for each of its units, and a launch holds
     // less than 2^32 threads.
-    KF_REQUIRE(max_q * (Hq / Hkv) <= kFewRows || prompt_plan(tokens, B, Hq, Hkv, D, max_ctx).units < 1 << 23,
+    KF_REQUIRE(max_q * (Hq / Hkv) <= kFewRows || prompt_units(tokens, B, Hq, Hkv) < 1 << 23,
                KF_E_UNSUPPORTED, "kf_paged_attention: too many requests of many rows");
     return KF_OK;
 }

@@ -403,14 +403,30 @@ constexpr int kUnitRows = PromptShape<128>::ROWS;
 
 }  // namespace
 
+int64_t prompt_units(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv) {
+    return (tokens * (Hq / Hkv) / kUnitRows + B) * Hkv;
+}
+
 PromptPlan prompt_plan(int64_t tokens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_ctx) {
     PromptPlan w;
     const int64_t rows = kUnitRows;
-    w.units = (tokens * (Hq / Hkv) / rows + B) * Hkv;
-    // Two workgroups a CU fit; fewer units than CUs have their keys split.
-    int64_t splits = w.units >= device_cu_count() ? 1 : (2 * device_cu_count() + w.units - 1) / w.units;
-    const int64_t most = max_ctx / 512;
+    w.units = prompt_units(tokens, B, Hq, Hkv);
+    // Two workgroups a CU fit; fewer units than CUs have their keys split over two
+    // a CU (us, split against whole, 32/8 heads of 128: 36 tokens over 30000 keys
+    // 66, 850; 512 over 30000 304, 764; 200 over 2000 33, 69).  260 units at a dim
+    // of 256 take 214 in two parts and 178 whole.  The parts are counted for units
+    // that are full, in one round of workgroups (200 tokens over 2000 keys, 9 parts
+    // of 56 units 33, 10 parts 41; four of 100 over 1000, 4 parts of 104 31, 5 parts
+    // 39; 12 ragged requests of 1 to 700, 2 parts of 188 94, 3 parts 92).
+    const int64_t full = ((tokens > 0 ? tokens : 1) * (Hq / Hkv) + rows - 1) / rows * Hkv;
+    int64_t splits = w.units >= device_cu_count() ? 1 : 2 * device_cu_count() / full;
+    // A part has at least so many keys (64 tokens over 1000 keys with 128, 256, 512:
+    // 18, 23, 35 us; at a dim of 256 300 tokens over 1000 keys 39, 33, 50).
+    const int64_t most = max_ctx / (D > 128 ? 256 : 128);
     if (splits > most) splits = most;
+    // Requests of few rows leave units empty: not more than 4 a CU, which bounds the
+    // workspace.
+    if (splits > 4 * device_cu_count() / w.units) splits = 4 * device_cu_count() / w.units;
     w.splits = splits > 1 ? (int)splits : 1;
     w.bytes = w.splits > 1 ? w.units * w.splits * rows * (D * 4 + 8) : 0;
     return w;

@@ -155,6 +155,33 @@ def test_c_entries_refuse_before_a_device():
     assert tab(total=(1 << 30) + 1) == 2
 
 
+def test_c_entries_refuse_what_no_launch_holds():
+    """A launch has less than 2^32 threads."""
+    lib = _lib.load()
+    null, some = ctypes.c_void_p(0), ctypes.c_void_p(16)
+    assert lib.kf_paged_cache_append(*[null] * 7, 1 << 27, 8, 2, 64, 16, 128, 64, 128, 64, _lib.KF_F16, 0, null) == 2
+    assert b"2^27" in lib.kf_last_error()
+    many = (1 << 22, 1 << 20, 8, 8, 64, 200, 64)  # tokens, requests, heads, key heads, dim, longest, context
+    assert lib.kf_paged_attention_workspace_bytes(*many) == -1
+    assert b"too many requests of many rows" in lib.kf_last_error()
+    assert lib.kf_paged_attention(*[null] * 7, some, *[null] * 3, 0, *many[:2], 8, 4, 8, 8, 64, 16, 512, 64, 200, 64, 0.1, 1,
+                                  3, _lib.KF_BF16, 1, null) == 2
+    assert lib.kf_paged_attention_workspace_bytes(4, 4, 4, 2, 64, 1 << 62, 64) == -1  # and no product wraps
+
+
+@pytest.mark.parametrize("max_query_len", [1, 128, 129, 4096])
+@pytest.mark.parametrize("Hq,Hkv,D", [(1, 1, 16), (32, 8, 128), (64, 1, 256)])
+def test_workspace_of_any_sound_shape(Hq, Hkv, D, max_query_len):
+    """Never negative, and at most four parts of 128 rows for each of 256 CUs,
+    whatever the lengths; no tokens included."""
+    lib = _lib.load()
+    for tokens in (0, 1, 127, 128, 129, 5000):
+        for B in (1, 3, 700):
+            for context in (0, 1, 128, 1024, 2049, 2 ** 31 - 1):
+                got = lib.kf_paged_attention_workspace_bytes(tokens, B, Hq, Hkv, D, max_query_len, context)
+                assert 0 <= got <= 4 * 256 * 128 * (D * 4 + 8)
+
+
 def test_bad_pages_lead_nowhere():
     """The index arithmetic of the kernels, on the host: no table entry, slot,
     start or length leads outside the arrays."""
