@@ -33,7 +33,7 @@ constexpr float kPScale = 32768.0f;  // 2^15, the largest f16 operand of the sec
 // ---------------------------------------------------------------------------
 template <int DP, int RT> struct RowsShape {
     // 16-key tiles of a turn: what two wavefronts a SIMD have registers for.
-        static constexpr int NT = DP * RT > 128 ? 2 : 4;
+    static constexpr int NT = DP * RT > 128 ? 2 : 4;
     static constexpr int KEYS = 16 * NT;            // keys a wavefront takes in a turn
     static constexpr int ROWS = 16 * RT;            // rows of a unit
     static constexpr int OC = DP < 128 ? DP : 128;  // columns joined at a time

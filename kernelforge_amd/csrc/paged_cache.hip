@@ -21,7 +21,10 @@ constexpr int kTokensPerThread = 4;
 // belongs to one of the call's tokens, so the token that stands there writes
 // the table entry and nothing has to loop over blocks.  Every workgroup sums
 // all lengths for itself (two scans over B values that the L2 holds) and then
-// handles its own tokens: one launch, no workspace.
+// handles its own tokens, four a thread so that a step of 2048 tokens is one
+// workgroup and may change the counts in place: one launch, no workspace.  Bound
+// by the latency of the lengths, the scans and the entries: 4.8 us for 64 requests
+// of one token, 5.9 us for 60000 tokens of 48 prompts.
 // ---------------------------------------------------------------------------
 struct TableParams {
     int* tables;
@@ -159,7 +162,10 @@ __global__ __launch_bounds__(kTableThreads) void paged_tables_kernel(TableParams
 // ballots over the slots of 64 tokens.  A unit is the block's keys or values of
 // one head, and each of its 16-token groups has a wavefront, so a unit's elements
 // stay in registers between the maximum that sets the scale and the rounding: the
-// call reads its inputs once and writes the codes once.
+// call reads its inputs once and writes the codes once.  17300 tokens of 8 heads
+// of 128 in blocks of 16 (107 MB) take 30 us, 3.5 TB/s, against 20 at a copy's
+// rate: a run's loads wait for the one before it.  64 tokens of 64 requests take
+// 6 us, which is latency (slots, scale, tokens, maximum).
 //
 // The scale is the least power of two s >= 2^-126 with max|x| <= M s (M the
 // largest code, 448 or 127) and never shrinks while the block fills.  x / s is
